@@ -9,6 +9,7 @@ cross the ABI as plain integers.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -29,6 +30,7 @@ MOE_ERR_BAD_OFFSETS = 7
 DT_BF16, DT_F16, DT_F32, DT_I8, DT_I32, DT_I64 = range(6)
 FFN_KERNEL_AUTO, FFN_KERNEL_TILED, FFN_KERNEL_STREAM, FFN_KERNEL_PAIR, FFN_KERNEL_WARP = range(5)
 ROUTER_SOFTMAX, ROUTER_SIGMOID_GROUP = 0, 1
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_FULL = range(4)
 
 _TORCH_DT = {
     torch.bfloat16: DT_BF16,
@@ -52,6 +54,14 @@ class MoeLayerDesc(ctypes.Structure):
         ("k", _i32), ("act_dtype", _i32), ("x_dtype", _i32), ("out_dtype", _i32), ("w_dtype", _i32),
         ("scale_dtype", _i32), ("router_mode", _i32), ("renorm", _i32), ("n_group", _i32),
         ("topk_group", _i32), ("routed_scaling", _f32), ("router_w_dtype", _i32),
+    ]
+
+
+class MoeNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("T", _i64), ("H", _i64), ("y_stride", _i64), ("res_stride", _i64), ("gate_stride", _i64),
+        ("y_dtype", _i32), ("res_dtype", _i32), ("post_dtype", _i32), ("next_dtype", _i32), ("gate_dtype", _i32),
+        ("norm_dtype", _i32), ("gate_mode", _i32), ("residual_scale", _f32), ("eps", _f32),
     ]
 
 
@@ -100,6 +110,18 @@ _SIGNATURES = {
     "moe_layer_forward": (
         [ctypes.POINTER(MoeLayerDesc), _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
          _p, _p, _sz, _p, _p],
+        _i32,
+    ),
+    "moe_permute_rows": ([_p, _i32, _i64, _p, _p, _i64, _i32, _i64, _i64, _p, _p, _p], _i32),
+    "moe_permute_rows_backward": ([_p, _i32, _i64, _p, _i64, _i32, _i64, _p, _i32, _p, _p], _i32),
+    "moe_combine_backward": (
+        [_p, _i32, _i64, _p, _i32, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _p, _p, _p, _p],
+        _i32,
+    ),
+    "moe_norm_gate_residual": ([ctypes.POINTER(MoeNormDesc), _p, _p, _p, _p, _p, _p, _p, _p], _i32),
+    "moe_norm_backward_workspace_bytes": ([_i64, _i64], _sz),
+    "moe_norm_gate_residual_backward": (
+        [ctypes.POINTER(MoeNormDesc), _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p],
         _i32,
     ),
     # include/moe_ep_b200.h
@@ -168,6 +190,29 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def device_guard(device: torch.device):
+    """Makes ``device`` current for the C call (the library launches on the
+    current device) when it is not already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def grad_wanted(what: str, *tensors: torch.Tensor | None) -> bool:
+    """Whether autograd has to record this call. Refused while a CUDA graph is
+    being captured: autograd's own stream bookkeeping for the leaves is not
+    part of the capture, and a captured backward of leaves that an eager graph
+    also holds ends the process. The explicit ``*_backward`` calls capture."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            f"{what}: autograd is not recorded during CUDA graph capture; call it under torch.no_grad() and use "
+            "the explicit backward function"
+        )
+    return True
 
 
 def check(rc: int, what: str) -> None:

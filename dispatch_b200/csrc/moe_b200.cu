@@ -21,6 +21,8 @@
 #include "gemm_stream.cuh"
 #include "gemm_warp.cuh"
 #include "group.cuh"
+#include "norm.cuh"
+#include "permute.cuh"
 #include "route.cuh"
 
 namespace {
@@ -1490,6 +1492,318 @@ int moe_ep_exchange(const int32_t* payload, int64_t n, void* const* peer_signal,
   p.status = status;
   CUDA_TRY(launch_pdl(moe::ep::exchange_kernel, dim3(1), dim3(256), 0, static_cast<cudaStream_t>(stream), p),
            "exchange_kernel launch");
+  return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- permute and combine gradients
+namespace {
+bool is_float(int dt) { return dt == MOE_DT_BF16 || dt == MOE_DT_F16 || dt == MOE_DT_F32; }
+
+// One thread per 8 columns of a row, at most 256.
+unsigned row_threads(int64_t H) {
+  const int64_t t = (H / 8 + 31) / 32 * 32;
+  return static_cast<unsigned>(t > moe::permute::kMaxThreads ? moe::permute::kMaxThreads : t);
+}
+
+int check_rows(const char* what, const void* rows, int dt, int64_t stride, int64_t H) {
+  CHECK_ARG(rows, "%s: null pointer", what);
+  CHECK_ARG(is_float(dt), "%s: dtype must be bf16, f16 or f32", what);
+  CHECK_ARG(aligned16(rows) && stride >= H && stride % 8 == 0,
+            "%s: rows must be 16-byte aligned, their stride a multiple of 8 and at least H", what);
+  return MOE_OK;
+}
+
+int check_slots(int64_t T, int k, int64_t H) {
+  CHECK_ARG(k >= 1 && k <= moe::permute::kMaxK, "top_k=%d must be in [1, %d]", k, moe::permute::kMaxK);
+  CHECK_ARG(T >= 0 && T * k < (1ll << 31), "T*k=%lld out of range", (long long)(T * k));
+  CHECK_ARG(H >= 8 && H % 8 == 0, "H=%lld must be a multiple of 8", (long long)H);
+  return MOE_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int moe_permute_rows(const void* x, int dtype, int64_t x_stride, const int32_t* pos, const int32_t* offsets,
+                     int64_t T, int k, int64_t E, int64_t H, void* xs, int32_t* status, void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  rc = check_slots(T, k, H);
+  if (rc || T == 0) return rc;
+  rc = check_rows("x", x, dtype, x_stride, H);
+  if (!rc) rc = check_rows("xs", xs, dtype, H, H);
+  if (rc) return rc;
+  CHECK_ARG(pos && offsets && E >= 1, "null grouping");
+  moe::permute::Params p{};
+  p.x = x;
+  p.out_rows = xs;
+  p.pos = pos;
+  p.n_rows = offsets + E;
+  p.status = status;
+  p.T = T;
+  p.H = H;
+  p.x_stride = x_stride;
+  p.k = k;
+  p.x_dt = dtype;
+  CUDA_TRY(launch_pdl(moe::permute::permute_kernel, dim3(static_cast<unsigned>(T)), dim3(row_threads(H)), 0,
+                      static_cast<cudaStream_t>(stream), p),
+           "permute_kernel launch");
+  return MOE_OK;
+}
+
+int moe_permute_rows_backward(const void* dxs, int dxs_dtype, int64_t dxs_stride, const int32_t* pos, int64_t T,
+                              int k, int64_t H, void* dx, int dx_dtype, int32_t* status, void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  rc = check_slots(T, k, H);
+  if (rc || T == 0) return rc;
+  rc = check_rows("dxs", dxs, dxs_dtype, dxs_stride, H);
+  if (!rc) rc = check_rows("dx", dx, dx_dtype, H, H);
+  if (rc) return rc;
+  CHECK_ARG(pos, "null grouping");
+  moe::permute::Params p{};
+  p.rows = dxs;
+  p.rows_dt = dxs_dtype;
+  p.rows_stride = dxs_stride;
+  p.out = dx;
+  p.out_dt = dx_dtype;
+  p.pos = pos;
+  p.status = status;
+  p.T = T;
+  p.H = H;
+  p.k = k;
+  CUDA_TRY(launch_pdl(moe::permute::permute_backward_kernel, dim3(static_cast<unsigned>(T)), dim3(row_threads(H)), 0,
+                      static_cast<cudaStream_t>(stream), p),
+           "permute_backward_kernel launch");
+  return MOE_OK;
+}
+
+int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, const void* y, int y_dtype,
+                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const float* topk_w,
+                         int64_t T, int k, int64_t E, int64_t H, void* dy, float* dw, int32_t* status,
+                         void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  rc = check_slots(T, k, H);
+  if (rc || T == 0 || (!dy && !dw)) return rc;
+  rc = check_rows("dout", dout, dout_dtype, dout_stride, H);
+  if (!rc && dw) rc = check_rows("y", y, y_dtype, y_stride, H);
+  if (!rc && dy) rc = check_rows("dy", dy, y_dtype, H, H);
+  if (rc) return rc;
+  CHECK_ARG(pos && offsets && topk_w && E >= 1, "null grouping");
+  moe::permute::Params p{};
+  p.x = dout;
+  p.x_dt = dout_dtype;
+  p.x_stride = dout_stride;
+  p.rows = y;
+  p.rows_dt = y_dtype;
+  p.rows_stride = y_stride;
+  p.out_rows = dy;
+  p.out_dt = y_dtype;
+  p.pos = pos;
+  p.n_rows = offsets + E;
+  p.w = topk_w;
+  p.dw = dw;
+  p.status = status;
+  p.T = T;
+  p.H = H;
+  p.k = k;
+  auto kernel = dw ? moe::permute::combine_backward_kernel<true> : moe::permute::combine_backward_kernel<false>;
+  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(T)), dim3(row_threads(H)), 0,
+                      static_cast<cudaStream_t>(stream), p),
+           "combine_backward_kernel launch");
+  return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- block norms
+namespace {
+using NormKernel = void (*)(const moe::norm::Params);
+
+// Slabs of partial column sums, at most: four CTAs on each of 148 SMs.
+constexpr int64_t kNormMaxSlabs = 592;
+
+struct NormShape {
+  int threads, rows_per_cta;
+  NormKernel forward, backward;
+};
+
+template <int kTpr, int kNv>
+NormShape norm_shape(bool vec) {
+  using G = moe::norm::Group<kTpr>;
+  NormShape s;
+  s.threads = G::kThreads;
+  s.rows_per_cta = G::kRpc;
+  s.forward = vec ? moe::norm::norm_forward_kernel<kTpr, kNv, true> : moe::norm::norm_forward_kernel<kTpr, kNv, false>;
+  s.backward =
+      vec ? moe::norm::norm_backward_kernel<kTpr, kNv, true> : moe::norm::norm_backward_kernel<kTpr, kNv, false>;
+  return s;
+}
+
+// Threads per row: the fewest of 32, 64, ... that hold H at 8 values each.
+NormShape norm_shape_for(int64_t H, bool vec) {
+  const int64_t v = (H + 7) / 8;
+  if (v <= 32) return norm_shape<32, 1>(vec);
+  if (v <= 64) return norm_shape<64, 1>(vec);
+  if (v <= 128) return norm_shape<128, 1>(vec);
+  if (v <= 256) return norm_shape<256, 1>(vec);
+  if (v <= 512) return norm_shape<512, 1>(vec);
+  if (v <= 1024) return norm_shape<1024, 1>(vec);
+  return norm_shape<1024, 2>(vec);
+}
+
+int norm_rows_per_cta(int64_t H) {
+  const int64_t v = (H + 7) / 8;
+  return v <= 32 ? 8 : v <= 64 ? 4 : v <= 128 ? 2 : 1;
+}
+
+int64_t norm_slabs(int64_t T, int64_t H) {
+  const int64_t rpc = norm_rows_per_cta(H);
+  const int64_t ctas = (T + rpc - 1) / rpc;
+  return ctas < kNormMaxSlabs ? ctas : kNormMaxSlabs;
+}
+
+int norm_params(const MoeNormDesc* d, const void* y, const void* residual, const void* post, const void* next,
+                const void* gate, moe::norm::Params* p, bool* vec) {
+  CHECK_ARG(d, "null descriptor");
+  CHECK_ARG(d->T >= 0 && d->T < (1ll << 31), "T=%lld out of range", (long long)d->T);
+  CHECK_ARG(d->H >= 1 && d->H <= moe::norm::kMaxH, "H=%lld must be in [1, %d]", (long long)d->H, moe::norm::kMaxH);
+  CHECK_ARG(d->gate_mode >= MOE_GATE_NONE && d->gate_mode <= MOE_GATE_FULL, "unknown gate mode %d", d->gate_mode);
+  CHECK_ARG(is_float(d->res_dtype) && (!y || is_float(d->y_dtype)) && (!post || is_float(d->post_dtype)) &&
+                (!next || (is_float(d->next_dtype) && is_float(d->norm_dtype))) &&
+                (d->gate_mode == MOE_GATE_NONE || is_float(d->gate_dtype)),
+            "dtypes must be bf16, f16 or f32");
+  CHECK_ARG(d->res_stride >= d->H && (!y || d->y_stride >= d->H) &&
+                (d->gate_mode != MOE_GATE_FULL || d->gate_stride >= d->H),
+            "row strides must be at least H");
+  if (d->T > 0) {  // empty tensors may come with null pointers
+    CHECK_ARG(y || (!post && d->gate_mode == MOE_GATE_NONE), "post_weight and gate need y");
+    CHECK_ARG(y || next, "nothing to compute: no y and no next_weight");
+    CHECK_ARG(residual && (d->gate_mode == MOE_GATE_NONE || gate), "null pointer");
+  }
+  *p = moe::norm::Params{};
+  p->y = y;
+  p->residual = residual;
+  p->post = post;
+  p->next = next;
+  p->gate = gate;
+  p->T = d->T;
+  p->H = static_cast<int>(d->H);
+  p->y_stride = d->y_stride;
+  p->res_stride = d->res_stride;
+  p->gate_stride = d->gate_stride;
+  p->y_dt = d->y_dtype;
+  p->res_dt = d->res_dtype;
+  p->post_dt = d->post_dtype;
+  p->next_dt = d->next_dtype;
+  p->gate_dt = d->gate_dtype;
+  p->norm_dt = d->norm_dtype;
+  p->gate_mode = d->gate_mode;
+  p->scale = d->residual_scale;
+  p->eps = d->eps;
+  // 16-byte accesses where every row starts on a 16-byte boundary
+  *vec = d->H % 8 == 0 && aligned16(residual) && d->res_stride % 8 == 0 && aligned16(post) && aligned16(next) &&
+         (!y || (aligned16(y) && d->y_stride % 8 == 0)) &&
+         (d->gate_mode == MOE_GATE_NONE || d->gate_mode == MOE_GATE_TOKEN || aligned16(gate)) &&
+         (d->gate_mode != MOE_GATE_FULL || d->gate_stride % 8 == 0);
+  return MOE_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int moe_norm_gate_residual(const MoeNormDesc* d, const void* y, const void* residual, const void* post_weight,
+                           const void* next_weight, const void* gate, void* out, void* normed, void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  moe::norm::Params p;
+  bool vec = false;
+  rc = norm_params(d, y, residual, post_weight, next_weight, gate, &p, &vec);
+  if (rc || d->T == 0) return rc;
+  CHECK_ARG((!y || out) && (!next_weight || normed), "null output pointer");
+  p.out = out;
+  p.normed = normed;
+  vec = vec && aligned16(out) && aligned16(normed);
+  const NormShape s = norm_shape_for(d->H, vec);
+  const int64_t grid = (d->T + s.rows_per_cta - 1) / s.rows_per_cta;
+  CUDA_TRY(launch_pdl(s.forward, dim3(static_cast<unsigned>(grid)), dim3(s.threads), 0,
+                      static_cast<cudaStream_t>(stream), p),
+           "norm_forward_kernel launch");
+  return MOE_OK;
+}
+
+size_t moe_norm_backward_workspace_bytes(int64_t T, int64_t H) {
+  if (T <= 0 || H <= 0) return 0;
+  return static_cast<size_t>(norm_slabs(T, H)) * 3 * static_cast<size_t>(H) * sizeof(float);
+}
+
+int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int64_t d_out_stride,
+                                    const void* d_normed, int64_t d_normed_stride, const void* y,
+                                    const void* residual, const void* post_weight, const void* next_weight,
+                                    const void* gate, void* d_y, void* d_residual, void* d_post, void* d_next,
+                                    void* d_gate, void* workspace, size_t workspace_bytes, void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  moe::norm::Params p;
+  bool vec = false;
+  rc = norm_params(d, y, residual, post_weight, next_weight, gate, &p, &vec);
+  if (rc) return rc;
+  CHECK_ARG((!d_out || d_out_stride >= d->H) && (!d_normed || (next_weight && d_normed_stride >= d->H)),
+            "d_out / d_normed strides must be at least H, d_normed needs next_weight");
+  CHECK_ARG((!d_y || y) && (!d_post || post_weight) && (!d_next || next_weight) &&
+                (!d_gate || d->gate_mode != MOE_GATE_NONE),
+            "a gradient of an absent input");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool channel_gate = d_gate && d->gate_mode == MOE_GATE_CHANNEL;
+  const bool sums = d_post || d_next || channel_gate;
+  if (d->T == 0) {  // no rows: the sums over rows are zero
+    if (d_post) CUDA_TRY(cudaMemsetAsync(d_post, 0, d->H * dt_size(d->post_dtype), s), "memset d_post");
+    if (d_next) CUDA_TRY(cudaMemsetAsync(d_next, 0, d->H * dt_size(d->next_dtype), s), "memset d_next");
+    if (channel_gate) CUDA_TRY(cudaMemsetAsync(d_gate, 0, d->H * dt_size(d->gate_dtype), s), "memset d_gate");
+    return MOE_OK;
+  }
+  CHECK_ARG(!sums || (workspace && aligned16(workspace) &&
+                      workspace_bytes >= moe_norm_backward_workspace_bytes(d->T, d->H)),
+            "workspace too small");
+  p.d_out = d_out;
+  p.d_normed = d_normed;
+  p.d_out_stride = d_out_stride;
+  p.d_normed_stride = d_normed_stride;
+  p.d_y = d_y;
+  p.d_residual = d_residual;
+  p.d_gate = channel_gate ? nullptr : d_gate;
+  p.part = sums ? static_cast<float*>(workspace) : nullptr;
+  p.want_post = d_post != nullptr;
+  p.want_next = d_next != nullptr;
+  p.want_gate = channel_gate;
+  vec = vec && aligned16(d_out) && (!d_out || d_out_stride % 8 == 0) && aligned16(d_normed) &&
+        (!d_normed || d_normed_stride % 8 == 0) && aligned16(d_y) && aligned16(d_residual) &&
+        (d->gate_mode != MOE_GATE_FULL || aligned16(d_gate));
+  const NormShape sh = norm_shape_for(d->H, vec);
+  const int64_t grid = norm_slabs(d->T, d->H);
+  CUDA_TRY(launch_pdl(sh.backward, dim3(static_cast<unsigned>(grid)), dim3(sh.threads), 0, s, p),
+           "norm_backward_kernel launch");
+  if (!sums) return MOE_OK;
+  moe::norm::ReduceParams r;
+  r.part = p.part;
+  r.out[0] = d_post;
+  r.out[1] = d_next;
+  r.out[2] = channel_gate ? d_gate : nullptr;
+  r.dt[0] = d->post_dtype;
+  r.dt[1] = d->next_dtype;
+  r.dt[2] = d->gate_dtype;
+  r.slabs = static_cast<int>(grid);
+  r.H = static_cast<int>(d->H);
+  CUDA_TRY(launch_pdl(moe::norm::norm_reduce_kernel, dim3(static_cast<unsigned>((d->H + 31) / 32), 3), dim3(256), 0,
+                      s, r),
+           "norm_reduce_kernel launch");
   return MOE_OK;
 }
 

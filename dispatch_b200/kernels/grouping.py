@@ -4,6 +4,8 @@ src/dispatch/kernels/grouping.py).
 ``group_tokens_by_expert`` is a stable counting sort in two launches (no host
 sync, no argsort); ``ungroup_and_combine`` is the deterministic weighted
 combine (f32 sum in slot order, one rounding) instead of ``index_add_``.
+``permute_tokens`` and ``combine_tokens`` are the same gather and combine for
+training: differentiable, with their gradients also as plain calls.
 """
 
 from __future__ import annotations
@@ -112,3 +114,168 @@ def ungroup_and_combine(
             f"grouping describes {grouping.sorted_token_idx.shape[0]}"
         )
     return combine(grouped_output, grouping.pos, grouping.flat_weight, num_tokens, grouping.top_k)
+
+
+# ---------------------------------------------------------------- with gradients
+def _check_grouping(what: str, grouping: TokenGrouping, rows: torch.Tensor | None, tokens: int | None) -> int:
+    """The token count of ``grouping``; raises if rows or tokens do not fit it."""
+    n = grouping.pos.numel()
+    t = n // grouping.top_k
+    if tokens is not None and tokens != t:
+        raise ValueError(f"{what}: {tokens} tokens, grouping describes {t}")
+    if rows is not None and rows.shape[0] != n:
+        raise ValueError(f"{what}: {rows.shape[0]} rows, grouping describes {n}")
+    return t
+
+
+def _row_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (N, H), copied only if its rows cannot be read in 16-byte pieces
+    where they lie (a last stride other than 1, unaligned or overlapping rows)."""
+    if t.dim() != 2:
+        raise ValueError(f"expected (rows, H), got {tuple(t.shape)}")
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _flat_weight(what: str, topk_weight: torch.Tensor | None, grouping: TokenGrouping) -> torch.Tensor:
+    if topk_weight is None:
+        return grouping.flat_weight
+    if topk_weight.numel() != grouping.pos.numel():
+        raise ValueError(f"{what}: topk_weight has {topk_weight.numel()} values, grouping describes {grouping.pos.numel()}")
+    return topk_weight.detach().reshape(-1).float()
+
+
+def _permute(x: torch.Tensor, grouping: TokenGrouping) -> torch.Tensor:
+    dev = L.require_cuda(x, grouping.pos, what="permute_tokens")
+    x = _row_view(x)
+    t = _check_grouping("permute_tokens", grouping, None, x.shape[0])
+    h = x.shape[1]
+    xs = torch.empty(t * grouping.top_k, h, dtype=x.dtype, device=dev)
+    with L.device_guard(dev):
+        rc = L.lib().moe_permute_rows(
+            x.data_ptr(), L.dt(x), _stride(x), grouping.pos.data_ptr(), grouping.offsets.data_ptr(), t,
+            grouping.top_k, grouping.offsets.numel() - 1, h, xs.data_ptr(), L.status_word(dev).data_ptr(),
+            L.stream_ptr(dev),
+        )
+    L.check(rc, "permute_tokens")
+    return xs
+
+
+def permute_tokens_backward(dxs: torch.Tensor, grouping: TokenGrouping, *,
+                            out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """dx[t] = sum over the token's slots of dxs[pos], in f32 in slot order,
+    rounded once to ``out_dtype`` (default: dxs' type)."""
+    dev = L.require_cuda(dxs, grouping.pos, what="permute_tokens_backward")
+    dxs = _row_view(dxs)
+    t = _check_grouping("permute_tokens_backward", grouping, dxs, None)
+    h = dxs.shape[1]
+    dx = torch.empty(t, h, dtype=out_dtype or dxs.dtype, device=dev)
+    with L.device_guard(dev):
+        rc = L.lib().moe_permute_rows_backward(
+            dxs.data_ptr(), L.dt(dxs), _stride(dxs), grouping.pos.data_ptr(), t, grouping.top_k, h, dx.data_ptr(),
+            L.dt(dx), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+        )
+    L.check(rc, "permute_tokens_backward")
+    return dx
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, grouping):
+        ctx.grouping, ctx.dtype = grouping, x.dtype
+        return _permute(x, grouping)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dxs):
+        return permute_tokens_backward(dxs, ctx.grouping, out_dtype=ctx.dtype), None
+
+
+def permute_tokens(x: torch.Tensor, grouping: TokenGrouping) -> torch.Tensor:
+    """xs[pos[t*k+s]] = x[t]: each token's row once per slot, in expert order
+    (T*k, H), in x's type (bf16, f16 or f32; H a multiple of 8, k <= 32). Rows
+    that no slot owns, at and after ``offsets[E]``, are zero. Differentiable
+    in x."""
+    if L.grad_wanted("permute_tokens", x):
+        return _Permute.apply(x, grouping)
+    return _permute(x, grouping)
+
+
+def _combine(y, grouping, topk_weight, y_shared, out_dtype) -> torch.Tensor:
+    dev = L.require_cuda(y, grouping.pos, topk_weight, y_shared, what="combine_tokens")
+    t = _check_grouping("combine_tokens", grouping, y, None if y_shared is None else y_shared.shape[0])
+    w = _flat_weight("combine_tokens", topk_weight, grouping)
+    if y_shared is not None and y_shared.dtype != y.dtype:
+        raise ValueError(f"dtype mismatch: y is {y.dtype}, y_shared is {y_shared.dtype}")
+    if y_shared is not None and y_shared.shape[1:] != y.shape[1:]:
+        raise ValueError(f"y_shared.shape {tuple(y_shared.shape)} does not match rows of {tuple(y.shape)}")
+    with L.device_guard(dev):
+        return combine(y.detach(), grouping.pos, w, t, grouping.top_k,
+                       None if y_shared is None else y_shared.detach(), out_dtype)
+
+
+def combine_tokens_backward(
+    dout: torch.Tensor, y: torch.Tensor, grouping: TokenGrouping, topk_weight: torch.Tensor | None = None, *,
+    need_y: bool = True, need_weight: bool = True,
+) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """The gradients (dy, dweight) of ``combine_tokens``: dy[pos[f]] = w[f] *
+    dout[f/k] in y's type, zero in rows that no slot owns; dweight (T, k) =
+    <dout[f/k], y[pos[f]]>, summed in f32, in topk_weight's type (f32 for the
+    grouping's own weights). y_shared's gradient is dout itself."""
+    dev = L.require_cuda(dout, y, grouping.pos, topk_weight, what="combine_tokens_backward")
+    y, dout = _row_view(y), _row_view(dout)
+    t = _check_grouping("combine_tokens_backward", grouping, y, dout.shape[0])
+    if dout.shape[1] != y.shape[1]:
+        raise ValueError(f"dout.shape {tuple(dout.shape)} does not match rows of {tuple(y.shape)}")
+    w = _flat_weight("combine_tokens_backward", topk_weight, grouping)
+    h, k = y.shape[1], grouping.top_k
+    dy = torch.empty(y.shape[0], h, dtype=y.dtype, device=dev) if need_y else None
+    dw = torch.empty(t, k, dtype=torch.float32, device=dev) if need_weight else None
+    with L.device_guard(dev):
+        rc = L.lib().moe_combine_backward(
+            dout.data_ptr(), L.dt(dout), _stride(dout), y.data_ptr(), L.dt(y), _stride(y), grouping.pos.data_ptr(),
+            grouping.offsets.data_ptr(), w.data_ptr(), t, k, grouping.offsets.numel() - 1, h, L.ptr(dy), L.ptr(dw),
+            L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+        )
+    L.check(rc, "combine_tokens_backward")
+    if dw is not None and topk_weight is not None:
+        dw = dw.to(topk_weight.dtype).view(topk_weight.shape)
+    return dy, dw
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, topk_weight, y_shared, grouping, out_dtype):
+        ctx.save_for_backward(y, topk_weight)
+        ctx.grouping = grouping
+        return _combine(y, grouping, topk_weight, y_shared, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        y, topk_weight = ctx.saved_tensors
+        need_y, need_w, need_shared = ctx.needs_input_grad[:3]
+        dy = dw = None
+        if need_y or need_w:
+            dy, dw = combine_tokens_backward(dout, y, ctx.grouping, topk_weight, need_y=need_y, need_weight=need_w)
+        return dy, dw, dout.to(y.dtype) if need_shared else None, None, None
+
+
+def combine_tokens(
+    y: torch.Tensor, grouping: TokenGrouping, topk_weight: torch.Tensor | None = None, *,
+    y_shared: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """out[t] = sum_s topk_weight[t, s] * y[pos[t*k+s]] (+ y_shared[t]), in f32
+    in slot order, rounded once to ``out_dtype`` (default: y's type): the
+    reference's ungroup_and_combine with the weights as an argument, so that
+    it is differentiable in y, topk_weight and y_shared. ``topk_weight``
+    None: the weights the grouping was made with (no gradient for them)."""
+    if L.grad_wanted("combine_tokens", y, topk_weight, y_shared):
+        return _Combine.apply(y, topk_weight, y_shared, grouping, out_dtype)
+    return _combine(y, grouping, topk_weight, y_shared, out_dtype)

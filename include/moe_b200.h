@@ -304,6 +304,71 @@ int moe_layer_forward(const MoeLayerDesc* d, const void* x, const void* router_w
                       int32_t* topk_idx, float* topk_w, int32_t* counts, int32_t* offsets, void* workspace,
                       size_t workspace_bytes, int32_t* status, void* stream);
 
+/*
+ * Row gather by a given grouping, and the gradients of the gather and of the
+ * combine (the reference's grouping.py:25-61 is forward only). pos (T*k) and
+ * offsets (E+1) are moe_group_tokens' outputs; k <= 32, H a multiple of 8,
+ * rows 16-byte aligned. Row strides are in elements (multiples of 8, >= H);
+ * outputs are contiguous. A slot with pos = -1 has no row: it adds nothing
+ * and its dw is 0. Rows at and after offsets[E] are written as zeros.
+ *   moe_permute_rows           xs[pos[t*k+s]] = x[t]            (same type)
+ *   moe_permute_rows_backward  dx[t] = sum_s dxs[pos[t*k+s]]    (slot order, f32, rounded once)
+ *   moe_combine_backward       dy[pos[f]] = topk_w[f] * dout[f/k]   (y_dtype; dy NULL: skipped)
+ *                              dw[f] = <dout[f/k], y[pos[f]]>       (f32; dw NULL: skipped, y may be NULL)
+ */
+int moe_permute_rows(const void* x, int dtype, int64_t x_stride, const int32_t* pos, const int32_t* offsets,
+                     int64_t T, int k, int64_t E, int64_t H, void* xs, int32_t* status, void* stream);
+int moe_permute_rows_backward(const void* dxs, int dxs_dtype, int64_t dxs_stride, const int32_t* pos, int64_t T,
+                              int k, int64_t H, void* dx, int dx_dtype, int32_t* status, void* stream);
+int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, const void* y, int y_dtype,
+                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const float* topk_w,
+                         int64_t T, int k, int64_t E, int64_t H, void* dy, float* dw, int32_t* status,
+                         void* stream);
+
+/*
+ * The norms before and after a block with the block's gate, residual scale
+ * and residual add; no counterpart in the reference, whose layer starts and
+ * ends inside the model's own block code. Per row, in f32, each output
+ * rounded once:
+ *   out = residual + residual_scale * gate * rmsnorm(y) * post_weight
+ *   normed = rmsnorm(out) * next_weight,  rmsnorm(v) = v * rsqrt(mean(v^2) + eps)
+ * y NULL: out = residual, only normed is written (the norm alone).
+ * post_weight NULL: y is not normed. next_weight NULL: no normed. gate: one
+ * value per channel (H), per token (T, stride gate_stride) or per value
+ * (T, H, row stride gate_stride). H in [1, 16384]; any row stride >= H, any
+ * alignment (rows whose H, strides and addresses allow 16-byte accesses use
+ * them). Types: bf16, f16 or f32 each; out has res_dtype. out and normed are
+ * contiguous (T, H).
+ */
+#define MOE_GATE_NONE 0
+#define MOE_GATE_CHANNEL 1
+#define MOE_GATE_TOKEN 2
+#define MOE_GATE_FULL 3
+typedef struct MoeNormDesc {
+  int64_t T, H;
+  int64_t y_stride, res_stride, gate_stride;
+  int y_dtype, res_dtype, post_dtype, next_dtype, gate_dtype, norm_dtype;
+  int gate_mode;
+  float residual_scale, eps;
+} MoeNormDesc;
+int moe_norm_gate_residual(const MoeNormDesc* d, const void* y, const void* residual, const void* post_weight,
+                           const void* next_weight, const void* gate, void* out, void* normed, void* stream);
+/*
+ * Its gradients from d_out (res_dtype) and d_normed (norm_dtype), row strides
+ * d_out_stride / d_normed_stride; either may be NULL (zero). d_y (y_dtype),
+ * d_residual (res_dtype), d_post / d_next (the weights' types, summed over the
+ * rows), d_gate (gate_dtype, in the gate's shape, contiguous): each may be NULL.
+ * The column sums go through f32 slabs in the workspace
+ * (moe_norm_backward_workspace_bytes, no initialisation), joined in a fixed
+ * order; no workspace is needed without d_post, d_next and a channel d_gate.
+ */
+size_t moe_norm_backward_workspace_bytes(int64_t T, int64_t H);
+int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int64_t d_out_stride,
+                                    const void* d_normed, int64_t d_normed_stride, const void* y,
+                                    const void* residual, const void* post_weight, const void* next_weight,
+                                    const void* gate, void* d_y, void* d_residual, void* d_post, void* d_next,
+                                    void* d_gate, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
