@@ -124,6 +124,17 @@ _SIGNATURES = {
         [ctypes.POINTER(MoeNormDesc), _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p],
         _i32,
     ),
+    "moe_int4_workspace_bytes": ([_i64, _i64, _i64, _i64], _sz),
+    "moe_grouped_gemm_int4": (
+        [_p, _i32, _i64, _i64, _p, _p, _i32, _i32, _i64, _i64, _p, _p, _i64, _p, _sz, _p, _p],
+        _i32,
+    ),
+    "moe_ffn_int4_workspace_bytes": ([_i64, _i64, _i64, _i64], _sz),
+    "moe_expert_ffn_int4": (
+        [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _sz, _p, _p],
+        _i32,
+    ),
+    "moe_quantize_int4": ([_p, _i32, _i64, _i64, _i64, _i32, _p, _p, _i32, _p], _i32),
     # include/moe_ep_b200.h
     "moe_peer_alloc": ([_sz, ctypes.POINTER(_p)], _i32),
     "moe_peer_free": ([_p], _i32),
@@ -237,6 +248,8 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     s = _status.get(idx)
     if s is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device must not be captured: make one before the capture")
         s = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
         _status[idx] = s
     return s
@@ -256,7 +269,11 @@ def workspace(device: torch.device, nbytes: int, tag: str) -> torch.Tensor:
     least ``nbytes`` long. Kernels use it as scratch within one call (the
     grouping's per-chunk histograms, the router's partial-logit slabs, the
     FFN's intermediate rows); caching per stream keeps calls on concurrent
-    streams from sharing it."""
+    streams from sharing it. A call that is being captured into a CUDA graph
+    gets a buffer of its own, uncached and uninitialised, from the graph's
+    memory: graphs captured on one stream may be replayed on several at once."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     key = (idx, stream_ptr(device), tag)
     buf = _workspaces.get(key)

@@ -21,6 +21,7 @@
 #include "gemm_stream.cuh"
 #include "gemm_warp.cuh"
 #include "group.cuh"
+#include "int4.cuh"
 #include "norm.cuh"
 #include "permute.cuh"
 #include "route.cuh"
@@ -1804,6 +1805,309 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
   CUDA_TRY(launch_pdl(moe::norm::norm_reduce_kernel, dim3(static_cast<unsigned>((d->H + 31) / 32), 3), dim3(256), 0,
                       s, r),
            "norm_reduce_kernel launch");
+  return MOE_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- 4-bit weights
+namespace {
+using Int4Kernel = void (*)(const moe::int4::Params);
+
+// Bytes of 16-bit weights made at a time for many rows per expert.
+constexpr int64_t kInt4ChunkBytes = 256ll << 20;
+// Shared memory of one direct CTA: two per SM, with room left for L1.
+constexpr size_t kInt4Smem = 96 * 1024;
+
+// One product: data1/scale1 are the up projection of a SwiGLU pair.
+struct Int4Spec {
+  const void* x;
+  int act_dtype;
+  int64_t M, K, E, N;
+  const void *data0, *scale0, *data1, *scale1;
+  int scale_dtype, group;
+  const int32_t* offsets;
+  void* out;
+  int64_t ldo;
+};
+
+int log2_of(int64_t v) {
+  int s = 0;
+  while ((1ll << s) < v) ++s;
+  return s;
+}
+
+bool int4_direct(int64_t M, int64_t E) { return M <= MOE_INT4_DIRECT_ROWS * E; }
+
+// Experts whose 16-bit weights (projections x N x K) are made at a time.
+int64_t int4_chunk(int64_t E, int64_t N, int64_t K, int projections) {
+  const int64_t per = N * K * 2 * projections;
+  const int64_t n = per > 0 ? kInt4ChunkBytes / per : E;
+  return n < 1 ? 1 : n > E ? E : n;
+}
+
+size_t int4_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int projections) {
+  if (M <= 0 || E <= 0 || N <= 0 || K <= 0 || int4_direct(M, E)) return 0;
+  // each projection's weights start 256-byte aligned
+  return static_cast<size_t>(projections) *
+         ((static_cast<size_t>(int4_chunk(E, N, K, projections)) * N * K * 2 + 255) & ~size_t(255));
+}
+
+int check_int4(const Int4Spec& s) {
+  CHECK_ARG(is16(s.act_dtype), "dtype mismatch: activations must be bf16 or f16");
+  CHECK_ARG(is_float(s.scale_dtype), "scale dtype must be f32, bf16 or f16");
+  CHECK_ARG(s.group == 32 || s.group == 64 || s.group == 128 || s.group == 256,
+            "group size %d must be 32, 64, 128 or 256", s.group);
+  CHECK_ARG(s.E >= 1 && s.E <= moe::int4::kMaxE, "expert count %lld not in [1, %d]", (long long)s.E,
+            moe::int4::kMaxE);
+  CHECK_ARG(s.K >= 8 && s.K % 8 == 0 && s.K < (1 << 30), "K mismatch: K=%lld must be a multiple of 8", (long long)s.K);
+  CHECK_ARG(s.N >= 1 && s.N < (1 << 30) && s.M >= 0 && s.M < (1ll << 31) && s.ldo >= s.N, "bad M/N/ldo");
+  if (s.M == 0) return MOE_OK;
+  CHECK_ARG(s.x && s.data0 && s.scale0 && s.offsets && s.out, "null pointer");
+  CHECK_ARG(aligned16(s.x) && aligned16(s.data0) && aligned16(s.scale0) && aligned16(s.data1) && aligned16(s.scale1),
+            "x, weights and scales must be 16-byte aligned");
+  return MOE_OK;
+}
+
+template <int kMt, int kNt, bool kSwiglu, bool kF16, bool kG32>
+int launch_int4(moe::int4::Params p, int64_t units, int sms, cudaStream_t stream) {
+  constexpr uint32_t fixed = moe::int4::fixed_smem<kMt, kNt>();
+  const uint32_t stage = moe::int4::Shape<kMt, kNt>::kDataStage +
+                         moe::int4::scale_stage_bytes(kMt, p.group_shift, p.scale_shift);
+  int64_t stages = (static_cast<int64_t>(kInt4Smem) - fixed) / stage;
+  stages = stages > moe::int4::kMaxStages ? moe::int4::kMaxStages : stages;
+  static_assert(fixed + 2 * (moe::int4::Shape<kMt, kNt>::kDataStage + kMt * 1024) <= kInt4Smem, "two stages fit");
+  p.stages = static_cast<int>(stages);
+  const auto kernel = moe::int4::int4_kernel<kMt, kNt, kSwiglu, kF16, kG32>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [&] {
+    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kInt4Smem));
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(int4)");
+  const int64_t grid = units < 2 * sms ? units : 2 * sms;
+  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(moe::int4::kThreads), fixed + stages * stage,
+                      stream, p),
+           "int4_kernel launch");
+  return MOE_OK;
+}
+
+template <bool kSwiglu, bool kF16, bool kG32>
+int launch_int4_shape(const moe::int4::Params& p, int64_t avg_rows, int sms, cudaStream_t stream) {
+  // at most this many (weight tile, token tile) pairs, in 16 x 8 tiles
+  const int64_t out_tiles = (kSwiglu ? 2 : 1) * static_cast<int64_t>(p.n16);
+  auto units = [&](int mt, int nt) {
+    const int64_t tok = p.M / (8 * nt) + (p.E < p.M ? p.E : p.M);
+    return tok * ((out_tiles + mt - 1) / mt);
+  };
+  if (avg_rows > 8) return launch_int4<2, 4, kSwiglu, kF16, kG32>(p, units(2, 4), sms, stream);
+  if (avg_rows > 4) return launch_int4<2, 2, kSwiglu, kF16, kG32>(p, units(2, 2), sms, stream);
+  if constexpr (!kSwiglu) {
+    if (units(2, 1) < 4 * sms) return launch_int4<1, 1, kSwiglu, kF16, kG32>(p, units(1, 1), sms, stream);
+  }
+  return launch_int4<2, 1, kSwiglu, kF16, kG32>(p, units(2, 1), sms, stream);
+}
+
+template <bool kSwiglu>
+int run_int4_direct(const Int4Spec& s, int sms, int32_t* status, cudaStream_t stream) {
+  moe::int4::Params p{};
+  p.data0 = static_cast<const uint8_t*>(s.data0);
+  p.data1 = static_cast<const uint8_t*>(s.data1);
+  p.scale0 = static_cast<const uint8_t*>(s.scale0);
+  p.scale1 = static_cast<const uint8_t*>(s.scale1);
+  p.x = static_cast<const uint16_t*>(s.x);
+  p.offsets = s.offsets;
+  p.out = static_cast<uint16_t*>(s.out);
+  p.status = status;
+  p.ldo = s.ldo;
+  p.M = static_cast<int>(s.M);
+  p.N = static_cast<int>(s.N);
+  p.K = static_cast<int>(s.K);
+  p.E = static_cast<int>(s.E);
+  p.n16 = static_cast<int>((s.N + 15) / 16);
+  p.kb = static_cast<int>((s.K + 63) / 64);
+  p.groups = static_cast<int>((s.K + s.group - 1) / s.group);
+  p.group_shift = log2_of(s.group);
+  p.scale_dt = s.scale_dtype;
+  p.scale_shift = s.scale_dtype == MOE_DT_F32 ? 2 : 1;
+  p.f16 = s.act_dtype == MOE_DT_F16;
+  const int64_t avg = (s.M + s.E - 1) / s.E;
+  if (p.f16)
+    return s.group == 32 ? launch_int4_shape<kSwiglu, true, true>(p, avg, sms, stream)
+                         : launch_int4_shape<kSwiglu, true, false>(p, avg, sms, stream);
+  return s.group == 32 ? launch_int4_shape<kSwiglu, false, true>(p, avg, sms, stream)
+                       : launch_int4_shape<kSwiglu, false, false>(p, avg, sms, stream);
+}
+
+int run_dequant(const Int4Spec& s, const void* data, const void* scale, int64_t e0, int64_t experts, void* out,
+                cudaStream_t stream) {
+  moe::int4::DequantParams p{};
+  p.N = static_cast<int>(s.N);
+  p.K = static_cast<int>(s.K);
+  p.n16 = static_cast<int>((s.N + 15) / 16);
+  p.kb = static_cast<int>((s.K + 63) / 64);
+  p.groups = static_cast<int>((s.K + s.group - 1) / s.group);
+  p.group_shift = log2_of(s.group);
+  p.scale_dt = s.scale_dtype;
+  p.scale_shift = s.scale_dtype == MOE_DT_F32 ? 2 : 1;
+  p.f16 = s.act_dtype == MOE_DT_F16;
+  p.data = static_cast<const uint8_t*>(data) + e0 * p.n16 * p.kb * moe::int4::kBlockBytes;
+  p.scale = static_cast<const uint8_t*>(scale) + ((e0 * p.n16 * p.groups * 16) << p.scale_shift);
+  p.offsets = s.offsets + e0;
+  p.out = static_cast<uint16_t*>(out);
+  const int64_t blocks = (static_cast<int64_t>(p.n16) * p.kb + 7) / 8;
+  CUDA_TRY(launch_pdl(moe::int4::dequant_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(experts)),
+                      dim3(256), 0, stream, p),
+           "dequant_kernel launch");
+  return MOE_OK;
+}
+
+int run_int4(const Int4Spec& s, void* workspace, size_t workspace_bytes, int32_t* status, cudaStream_t stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  rc = check_int4(s);
+  if (rc || s.M == 0) return rc;
+  const bool swiglu = s.data1 != nullptr;
+  if (int4_direct(s.M, s.E))
+    return swiglu ? run_int4_direct<true>(s, sms, status, stream) : run_int4_direct<false>(s, sms, status, stream);
+  const int projections = swiglu ? 2 : 1;
+  const size_t need = int4_bytes(s.M, s.E, s.N, s.K, projections);
+  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace too small (%zu < %zu)",
+            workspace_bytes, need);
+  const int64_t chunk = int4_chunk(s.E, s.N, s.K, projections);
+  void* w0 = workspace;
+  void* w1 = static_cast<char*>(workspace) + need / projections;
+  for (int64_t e0 = 0; e0 < s.E; e0 += chunk) {
+    const int64_t n = s.E - e0 < chunk ? s.E - e0 : chunk;
+    rc = run_dequant(s, s.data0, s.scale0, e0, n, w0, stream);
+    if (!rc && swiglu) rc = run_dequant(s, s.data1, s.scale1, e0, n, w1, stream);
+    if (rc) return rc;
+    SegSpec g{};
+    g.a = s.x;
+    g.a_rows = s.M;
+    g.lda = s.K;
+    g.b0 = w0;
+    g.b1 = swiglu ? w1 : nullptr;
+    g.b_dtype = s.act_dtype;
+    g.G = n;
+    g.N = s.N;
+    g.K = s.K;
+    g.offsets = s.offsets + e0;
+    g.out = s.out;
+    g.ldo = s.ldo;
+    g.swiglu = swiglu;
+    const int pick = ffn_auto_kernel(s.M, s.E, 0, s.K, s.N, s.act_dtype, false);
+    rc = pick == MOE_FFN_KERNEL_PAIR ? run_gemm_pair(&g, 1, s.act_dtype, status, stream)
+                                     : run_gemm(&g, 1, s.act_dtype, status, stream);
+    if (rc) return rc;
+  }
+  return MOE_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K) { return int4_bytes(M, E, N, K, 1); }
+
+int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, const void* data, const void* scale,
+                          int scale_dtype, int group, int64_t E, int64_t N, const int32_t* offsets, void* out,
+                          int64_t ldo, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  Int4Spec s{};
+  s.x = x;
+  s.act_dtype = x_dtype;
+  s.M = M;
+  s.K = K;
+  s.E = E;
+  s.N = N;
+  s.data0 = data;
+  s.scale0 = scale;
+  s.scale_dtype = scale_dtype;
+  s.group = group;
+  s.offsets = offsets;
+  s.out = out;
+  s.ldo = ldo;
+  return run_int4(s, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I) {
+  if (R <= 0 || I <= 0) return 0;
+  const size_t a = int4_bytes(R, E, I, H, 2), b = int4_bytes(R, E, H, I, 1);
+  return ((static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255)) + (a > b ? a : b);
+}
+
+int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, const int32_t* offsets, int64_t E,
+                        int64_t I, const void* gate, const void* gate_scale, const void* up, const void* up_scale,
+                        const void* down, const void* down_scale, int scale_dtype, int group, void* y,
+                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  if (R == 0) return MOE_OK;
+  CHECK_ARG(gate && up && down, "null pointer");
+  CHECK_ARG(I >= 8 && I % 8 == 0, "I=%lld must be a multiple of 8", (long long)I);
+  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= moe_ffn_int4_workspace_bytes(R, E, H, I),
+            "workspace too small");
+  const size_t h_bytes = (static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255);
+  char* rest = static_cast<char*>(workspace) + h_bytes;
+  const size_t rest_bytes = workspace_bytes - h_bytes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Int4Spec s{};
+  s.x = xs;
+  s.act_dtype = act_dtype;
+  s.M = R;
+  s.K = H;
+  s.E = E;
+  s.N = I;
+  s.data0 = gate;
+  s.scale0 = gate_scale;
+  s.data1 = up;
+  s.scale1 = up_scale;
+  s.scale_dtype = scale_dtype;
+  s.group = group;
+  s.offsets = offsets;
+  s.out = workspace;
+  s.ldo = I;
+  int rc = run_int4(s, rest, rest_bytes, status, st);
+  if (rc) return rc;
+  s.x = workspace;
+  s.K = I;
+  s.N = H;
+  s.data0 = down;
+  s.scale0 = down_scale;
+  s.data1 = s.scale1 = nullptr;
+  s.out = y;
+  s.ldo = H;
+  return run_int4(s, rest, rest_bytes, status, st);
+}
+
+int moe_quantize_int4(const void* w, int w_dtype, int64_t E, int64_t N, int64_t K, int group, void* data,
+                      void* scale, int scale_dtype, void* stream) {
+  int sms = 0;
+  int rc = device_info(&sms);
+  if (rc) return rc;
+  CHECK_ARG(is_float(w_dtype), "bad weight dtype");
+  CHECK_ARG(is_float(scale_dtype), "bad scale dtype");
+  CHECK_ARG(group == 32 || group == 64 || group == 128 || group == 256, "group size %d must be 32, 64, 128 or 256",
+            group);
+  CHECK_ARG(E >= 0 && N >= 0 && K >= 0 && N < (1 << 30) && K < (1 << 30), "bad E/N/K");
+  if (E == 0 || N == 0 || K == 0) return MOE_OK;
+  CHECK_ARG(w && data && scale && aligned16(data), "null or unaligned pointer");
+  moe::int4::QuantParams p;
+  p.w = w;
+  p.data = static_cast<uint8_t*>(data);
+  p.scale = scale;
+  p.w_dt = w_dtype;
+  p.scale_dt = scale_dtype;
+  p.E = E;
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.n16 = static_cast<int>((N + 15) / 16);
+  p.kb = static_cast<int>((K + 63) / 64);
+  p.groups = static_cast<int>((K + group - 1) / group);
+  p.group = group;
+  const int64_t ctas = (E * p.n16 * p.groups + 7) / 8;
+  CHECK_ARG(ctas < (1ll << 31), "too many groups");
+  CUDA_TRY(launch_pdl(moe::int4::quantize_kernel, dim3(static_cast<unsigned>(ctas)), dim3(256), 0,
+                      static_cast<cudaStream_t>(stream), p),
+           "quantize_kernel launch");
   return MOE_OK;
 }
 

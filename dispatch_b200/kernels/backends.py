@@ -20,7 +20,12 @@ def resolve_backend(name: str) -> GroupedMatmul:
     return grouped_matmul
 
 
-def resolve_quantized_backend() -> QuantizedGroupedMatmul:
+def resolve_quantized_backend(bits: int = 8) -> QuantizedGroupedMatmul:
+    """``bits`` 8: per-channel int8 (the reference's), 4: int4 with group scales."""
+    from dispatch_b200.kernels.grouped_gemm_int4 import grouped_matmul_int4  # noqa: PLC0415
     from dispatch_b200.kernels.grouped_gemm_int8 import grouped_matmul_int8  # noqa: PLC0415
 
-    return grouped_matmul_int8
+    backends = {8: grouped_matmul_int8, 4: grouped_matmul_int4}
+    if bits not in backends:
+        raise ValueError(f"no quantised backend with {bits} bits; expected one of {tuple(backends)}")
+    return backends[bits]

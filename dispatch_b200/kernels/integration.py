@@ -14,6 +14,7 @@ from dispatch_b200.kernels.quantization import (
     QuantizedStackedExpertWeights,
     grouped_moe_routed_quantized,
     quantize_stacked_weights,
+    quantize_stacked_weights_int4,
 )
 
 MoEInfer = Callable[[torch.Tensor, torch.Tensor, torch.Tensor], torch.Tensor]
@@ -43,13 +44,22 @@ def patch_moe_infer(model: torch.nn.Module, matmul=None, *, block_m: int = 16) -
 
 
 def patch_moe_infer_quantized(model: torch.nn.Module, matmul=None, *, block_m: int = 16,
-                              scale_dtype: torch.dtype = torch.float32) -> int:
-    """Quantises each layer's stacked weights to int8 once, frees the
-    originals, and installs the int8 path."""
+                              scale_dtype: torch.dtype = torch.float32, bits: int = 8,
+                              group_size: int = 128) -> int:
+    """Quantises each layer's stacked weights once, to int8 per channel or
+    (``bits`` 4) to int4 in groups of ``group_size`` columns, frees the
+    originals, and installs the quantised path."""
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
     model.eval()
     patched = 0
     for module, experts in _iter_validated_moe_layers(model):
-        qweights = quantize_stacked_weights(stack_expert_weights(experts), scale_dtype=scale_dtype)
+        stacked = stack_expert_weights(experts)
+        if bits == 4:
+            qweights = quantize_stacked_weights_int4(stacked, group_size=group_size, scale_dtype=scale_dtype)
+        else:
+            qweights = quantize_stacked_weights(stacked, scale_dtype=scale_dtype)
+        del stacked
         _free_expert_weights(experts)
         module.moe_infer = _grouped_moe_infer_quantized(qweights, matmul, block_m)  # type: ignore[assignment]
         patched += 1

@@ -14,8 +14,10 @@ from dataclasses import dataclass
 import torch
 
 from dispatch_b200 import _lib as L
-from dispatch_b200.kernels.moe_forward import SharedExpertWeights, StackedExpertWeights, act_dtype_for
-from dispatch_b200.kernels.quantization import QuantizedStackedExpertWeights
+from dispatch_b200.kernels.block import norm_gate_residual, rms_norm
+from dispatch_b200.kernels.grouping import _group, combine
+from dispatch_b200.kernels.moe_forward import SharedExpertWeights, StackedExpertWeights, act_dtype_for, expert_ffn
+from dispatch_b200.kernels.quantization import Int4StackedExpertWeights, QuantizedStackedExpertWeights
 
 
 @dataclass(frozen=True)
@@ -40,7 +42,7 @@ class LayerOutput:
 def moe_layer_forward(
     x: torch.Tensor,
     router_weight: torch.Tensor | None,
-    weights: StackedExpertWeights | QuantizedStackedExpertWeights,
+    weights: StackedExpertWeights | QuantizedStackedExpertWeights | Int4StackedExpertWeights,
     router: RouterConfig,
     *,
     shared: SharedExpertWeights | None = None,
@@ -51,6 +53,8 @@ def moe_layer_forward(
     """x (T, H) bf16/f16 (or f32 with bf16 weights and no shared expert);
     router_weight (E, H) bf16/f32; ``topk`` = (idx int32 (T,k), w f32 (T,k))
     skips the router (the moe_infer contract)."""
+    if isinstance(weights, Int4StackedExpertWeights):
+        return _layer_int4(x, router_weight, weights, router, shared, e_score_bias, topk, out_dtype)
     quant = isinstance(weights, QuantizedStackedExpertWeights)
     g = weights.gate.data if quant else weights.gate
     u = weights.up.data if quant else weights.up
@@ -105,6 +109,74 @@ def moe_layer_forward(
     )
     L.check(rc, "moe_layer_forward")
     return LayerOutput(out, idx, wts, counts, offsets)
+
+
+def _layer_int4(x, router_weight, weights, router, shared, e_score_bias, topk, out_dtype) -> LayerOutput:
+    """The layer with 4-bit experts: the same route, grouping and combine
+    kernels around the int4 products, call by call."""
+    act = act_dtype_for(x, weights)
+    if shared is not None and x.dtype != act:
+        raise ValueError("the shared expert needs x in the activation dtype")
+    t, k = x.shape[0], router.top_k
+    if topk is None:
+        idx, wts = route(x, router_weight, router, e_score_bias=e_score_bias)
+    else:
+        idx, wts = topk[0].to(torch.int32).contiguous(), topk[1].to(torch.float32).contiguous()
+    x = x.contiguous()
+    counts, offsets, pos, _, _, w, xs = _group(idx, wts, weights.num_experts, x=x, xs_dtype=act, want_sorted=False)
+    y, ys = expert_ffn(xs, offsets, weights, shared, x if shared is not None else None)
+    out = combine(y, pos, w.reshape(-1), t, k, ys, out_dtype=out_dtype or x.dtype)
+    return LayerOutput(out, idx, wts, counts, offsets)
+
+
+@dataclass(frozen=True)
+class BlockOutput:
+    out: torch.Tensor  # the residual stream after the block
+    normed: torch.Tensor | None  # the next block's input, if next_weight was given
+    layer: LayerOutput
+
+
+def moe_block_forward(  # noqa: PLR0913
+    x: torch.Tensor,
+    pre_weight: torch.Tensor | None,
+    router_weight: torch.Tensor | None,
+    weights: StackedExpertWeights | QuantizedStackedExpertWeights | Int4StackedExpertWeights,
+    router: RouterConfig,
+    *,
+    normed: torch.Tensor | None = None,
+    post_weight: torch.Tensor | None = None,
+    next_weight: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    residual_scale: float = 1.0,
+    eps: float = 1e-6,
+    act_dtype: torch.dtype | None = None,
+    shared: SharedExpertWeights | None = None,
+    e_score_bias: torch.Tensor | None = None,
+    topk: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> BlockOutput:
+    """The MoE layer with the norms around it, for inference:
+
+        h   = rms_norm(x, pre_weight)          (or ``normed``, what the block before returned)
+        y   = moe_layer_forward(h, ...)
+        out = x + residual_scale * gate * rms_norm(y, post_weight)
+        normed = rms_norm(out, next_weight)    (if next_weight is given)
+
+    x (T, H) is the residual stream, bf16, f16 or f32; h and y are in
+    ``act_dtype`` (default: x's type, or for an f32 stream the weights' type,
+    bf16 for quantised ones). post_weight and gate as in
+    ``norm_gate_residual``."""
+    if (normed is None) == (pre_weight is None):
+        raise ValueError("give pre_weight or normed, not both")
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, pre_weight, normed, post_weight, next_weight, gate)):
+        raise ValueError("moe_block_forward is for inference: call it under torch.no_grad()")
+    if act_dtype is None:
+        act_dtype = x.dtype if x.dtype != torch.float32 else act_dtype_for(x, weights)
+    h = normed if normed is not None else rms_norm(x, pre_weight, eps=eps, out_dtype=act_dtype)
+    layer = moe_layer_forward(h, router_weight, weights, router, shared=shared, e_score_bias=e_score_bias, topk=topk)
+    out, nxt = norm_gate_residual(layer.out, x, post_weight, next_weight, gate=gate, residual_scale=residual_scale,
+                                  eps=eps, norm_dtype=act_dtype)
+    return BlockOutput(out, nxt, layer)
 
 
 def route(
@@ -181,9 +253,10 @@ class CapturedLayer:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=self.stream):
             self.result = moe_layer_forward(self.x, *self._args, **self._kw)
-        # the graph holds raw pointers into this stream's cached workspaces: keep them alive
+        # the captured call's workspaces are the graph's own; the warm-up's are done with
         sid = self.stream.cuda_stream
-        self._keep = [buf for (_, s, _), buf in L._workspaces.items() if s == sid]
+        for key in [key for key in L._workspaces if key[1] == sid]:
+            del L._workspaces[key]
         torch.cuda.current_stream(dev).wait_stream(self.stream)
 
     def replay(self) -> LayerOutput:

@@ -103,11 +103,17 @@ def expert_ffn(xs: torch.Tensor, offsets: torch.Tensor, weights, shared: SharedE
                n_rows: int | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """y = down(silu(gate(xs)) * up(xs)) per expert group, and the shared
     expert over x_shared, in two tcgen05 launches. ``weights`` is a
-    StackedExpertWeights (bf16/f16) or a QuantizedStackedExpertWeights.
+    StackedExpertWeights (bf16/f16), a QuantizedStackedExpertWeights or an
+    Int4StackedExpertWeights (without ``gather_rows``).
     With ``gather_rows`` (int64, n_rows entries) routed row r is row
     gather_rows[r] of ``xs``, fetched by the GEMM's TMA gather instead of a copy."""
-    from dispatch_b200.kernels.quantization import QuantizedStackedExpertWeights  # noqa: PLC0415
+    from dispatch_b200.kernels.quantization import (  # noqa: PLC0415
+        Int4StackedExpertWeights,
+        QuantizedStackedExpertWeights,
+    )
 
+    if isinstance(weights, Int4StackedExpertWeights):
+        return _expert_ffn_int4(xs, offsets, weights, shared, x_shared, gather_rows)
     quant = isinstance(weights, QuantizedStackedExpertWeights)
     g, u, d = (weights.gate.data, weights.up.data, weights.down.data) if quant else (weights.gate, weights.up, weights.down)
     dev = L.require_cuda(xs, offsets, g, u, d, x_shared, gather_rows, what="the B200 expert FFN")
@@ -158,11 +164,43 @@ def expert_ffn(xs: torch.Tensor, offsets: torch.Tensor, weights, shared: SharedE
     return y, ys
 
 
+def _expert_ffn_int4(xs, offsets, weights, shared: SharedExpertWeights | None, x_shared, gather_rows):
+    """The 4-bit routed experts, and the shared expert (in the activation type)
+    in launches of its own."""
+    from dispatch_b200.kernels.grouped_gemm_int4 import expert_ffn_int4  # noqa: PLC0415
+
+    if gather_rows is not None:
+        raise ValueError("int4 experts take no gathered rows")
+    y = expert_ffn_int4(xs, offsets, weights)
+    if shared is None:
+        return y, None
+    if x_shared is None:
+        raise ValueError("shared expert needs x_shared")
+    act, h = xs.dtype, xs.shape[1]
+    if shared.gate.dtype != act or x_shared.dtype != act:
+        raise ValueError(f"dtype mismatch: shared expert must be {act}")
+    dev = L.require_cuda(xs, x_shared, shared.gate, shared.up, shared.down, what="the B200 expert FFN")
+    t, i_sh = x_shared.shape[0], shared.gate.shape[0]
+    ys = torch.empty(t, h, dtype=act, device=dev)
+    lib = L.lib()
+    ws = torch.empty(max(lib.moe_ffn_workspace_bytes(0, 0, t, i_sh), 256), dtype=torch.uint8, device=dev)
+    x_shared = x_shared.contiguous()
+    gate, up, down = shared.gate.contiguous(), shared.up.contiguous(), shared.down.contiguous()
+    with L.device_guard(dev):
+        rc = lib.moe_expert_ffn_grouped(
+            3, None, L.dt(act), 0, h, None, 1, 1, None, 0, 0, None, None, None, L.dt(act), None, None, None, 0,
+            x_shared.data_ptr(), t, i_sh, gate.data_ptr(), up.data_ptr(), down.data_ptr(), None, ys.data_ptr(),
+            ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+        )
+    L.check(rc, "expert_ffn")
+    return y, ys
+
+
 def act_dtype_for(x: torch.Tensor, weights) -> torch.dtype:
-    """The tensor-core input type: the weights' type, or for int8 weights the
-    activation type (bf16 when x is f32)."""
+    """The tensor-core input type: the weights' type, or for int8 and int4
+    weights the activation type (bf16 when x is f32)."""
     gate = getattr(weights.gate, "data", weights.gate)
-    if gate.dtype == torch.int8:
+    if gate.dtype in (torch.int8, torch.int32):
         return x.dtype if x.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
     return gate.dtype
 

@@ -369,6 +369,49 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
                                     const void* gate, void* d_y, void* d_residual, void* d_post, void* d_next,
                                     void* d_gate, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Expert products with 4-bit weights and group scales (beside the int8 ones;
+ * no reference counterpart): out[r, n] = sum_k x[r, k] * code[e, n, k] *
+ * scale[e, n, k / group] for the rows r of expert e, codes -8..7, f32
+ * accumulation. group: 32, 64, 128 or 256 columns; K a multiple of 8, any N.
+ *
+ * Laid out weights (16-byte aligned): with n16 = ceil(N/16), kb = ceil(K/64),
+ * groups = ceil(K/group),
+ *   data   (E, n16, kb, 32 lanes, 4) int32: nibble (4 h + 8 p + 16 c) of word
+ *          2 j + s of lane 4 g + q holds code + 8 of row 16 i + 8 h + g, column
+ *          64 b + 32 j + 8 q + 4 s + 2 p + c; rows >= N and columns >= K hold 8;
+ *   scale  (E, n16, groups, 16) in scale_dtype (f32, bf16 or f16).
+ * moe_quantize_int4 makes both from w (E, N, K): per row and group scale =
+ * absmax / 7 in f32 (1 for a group of zeros) rounded to scale_dtype, code =
+ * clamp(round_half_even(w / scale), -8, 7).
+ *
+ * Groups averaging at most MOE_INT4_DIRECT_ROWS rows multiply the codes
+ * themselves (no weight is rounded, no workspace). Beyond that the weights of
+ * as many experts as fit the workspace at a time are written as code * scale
+ * rounded to x's type and multiplied on the tcgen05 kernels; f16 then holds
+ * them in f16's range, as it does f16 weights. workspace:
+ * moe_int4_workspace_bytes (0 for a direct call), 16-byte aligned, no
+ * initialisation. x (M, K) and out (M, ldo) bf16 or f16.
+ */
+#define MOE_INT4_DIRECT_ROWS 32
+size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K);
+int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, const void* data, const void* scale,
+                          int scale_dtype, int group, int64_t E, int64_t N, const int32_t* offsets, void* out,
+                          int64_t ldo, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/*
+ * The expert FFN over grouped rows with 4-bit weights, as moe_expert_ffn:
+ * y = (silu(xs gate^T) * (xs up^T)) down^T, gate/up (E, I, H) and down
+ * (E, H, I) laid out, one group size and scale type for the three. The
+ * intermediate rows are in xs' type (in the workspace), SwiGLU in f32.
+ */
+size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I);
+int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, const int32_t* offsets, int64_t E,
+                        int64_t I, const void* gate, const void* gate_scale, const void* up, const void* up_scale,
+                        const void* down, const void* down_scale, int scale_dtype, int group, void* y,
+                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int moe_quantize_int4(const void* w, int w_dtype, int64_t E, int64_t N, int64_t K, int group, void* data,
+                      void* scale, int scale_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
