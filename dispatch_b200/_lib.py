@@ -9,7 +9,6 @@ cross the ABI as plain integers.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -113,15 +112,18 @@ _SIGNATURES = {
         _i32,
     ),
     "moe_permute_rows": ([_p, _i32, _i64, _p, _p, _i64, _i32, _i64, _i64, _p, _p, _p], _i32),
-    "moe_permute_rows_backward": ([_p, _i32, _i64, _p, _i64, _i32, _i64, _p, _i32, _p, _p], _i32),
+    "moe_unpermute_rows": (
+        [_p, _i32, _i64, _p, _p, _i32, _p, _i64, _i64, _i32, _i64, _p, _i32, _p, _p],
+        _i32,
+    ),
     "moe_combine_backward": (
-        [_p, _i32, _i64, _p, _i32, _i64, _p, _p, _p, _i64, _i32, _i64, _i64, _p, _p, _p, _p],
+        [_p, _i32, _i64, _p, _i32, _i64, _p, _p, _p, _i32, _i64, _i32, _i64, _i64, _p, _p, _p, _p],
         _i32,
     ),
     "moe_norm_gate_residual": ([ctypes.POINTER(MoeNormDesc), _p, _p, _p, _p, _p, _p, _p, _p], _i32),
     "moe_norm_backward_workspace_bytes": ([_i64, _i64], _sz),
     "moe_norm_gate_residual_backward": (
-        [ctypes.POINTER(MoeNormDesc), _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p],
+        [ctypes.POINTER(MoeNormDesc), _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p],
         _i32,
     ),
     "moe_int4_workspace_bytes": ([_i64, _i64, _i64, _i64], _sz),
@@ -200,15 +202,22 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle: torch.cuda.current_stream() builds a Stream object for it,
+    # 2.3 us of host time per call against 0.1
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(idx)
 
 
-def device_guard(device: torch.device):
-    """Makes ``device`` current for the C call (the library launches on the
-    current device) when it is not already."""
+def call(what: str, device: torch.device, fn, *args) -> None:
+    """``fn(*args)`` with ``device`` current (the library launches on the
+    current device), its status raised as ``check`` does."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args)
+    if rc != MOE_OK:
+        check(rc, what)
 
 
 def grad_wanted(what: str, *tensors: torch.Tensor | None) -> bool:

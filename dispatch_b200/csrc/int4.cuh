@@ -51,13 +51,6 @@ struct Params {
   int f16, stages;
 };
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // The A operand of one MMA step from its word of eight codes.
 template <bool kF16>
 __device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4]) {

@@ -1554,37 +1554,46 @@ int moe_permute_rows(const void* x, int dtype, int64_t x_stride, const int32_t* 
   return MOE_OK;
 }
 
-int moe_permute_rows_backward(const void* dxs, int dxs_dtype, int64_t dxs_stride, const int32_t* pos, int64_t T,
-                              int k, int64_t H, void* dx, int dx_dtype, int32_t* status, void* stream) {
+int moe_unpermute_rows(const void* rows, int rows_dtype, int64_t rows_stride, const int32_t* pos, const void* w,
+                       int w_dtype, const void* shared, int64_t shared_stride, int64_t T, int k, int64_t H,
+                       void* out, int out_dtype, int32_t* status, void* stream) {
   int sms = 0;
   int rc = device_info(&sms);
   if (rc) return rc;
   rc = check_slots(T, k, H);
   if (rc || T == 0) return rc;
-  rc = check_rows("dxs", dxs, dxs_dtype, dxs_stride, H);
-  if (!rc) rc = check_rows("dx", dx, dx_dtype, H, H);
+  rc = check_rows("rows", rows, rows_dtype, rows_stride, H);
+  if (!rc) rc = check_rows("out", out, out_dtype, H, H);
+  if (!rc && shared) rc = check_rows("shared", shared, rows_dtype, shared_stride, H);
   if (rc) return rc;
   CHECK_ARG(pos, "null grouping");
+  CHECK_ARG(!w || is_float(w_dtype), "weights: dtype must be bf16, f16 or f32");
   moe::permute::Params p{};
-  p.rows = dxs;
-  p.rows_dt = dxs_dtype;
-  p.rows_stride = dxs_stride;
-  p.out = dx;
-  p.out_dt = dx_dtype;
+  p.rows = rows;
+  p.rows_dt = rows_dtype;
+  p.rows_stride = rows_stride;
+  p.x = shared;
+  p.x_dt = rows_dtype;
+  p.x_stride = shared_stride;
+  p.w = w;
+  p.w_dt = w_dtype;
+  p.out = out;
+  p.out_dt = out_dtype;
   p.pos = pos;
   p.status = status;
   p.T = T;
   p.H = H;
   p.k = k;
-  CUDA_TRY(launch_pdl(moe::permute::permute_backward_kernel, dim3(static_cast<unsigned>(T)), dim3(row_threads(H)), 0,
+  auto kernel = w ? moe::permute::unpermute_kernel<true> : moe::permute::unpermute_kernel<false>;
+  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(T)), dim3(row_threads(H)), 0,
                       static_cast<cudaStream_t>(stream), p),
-           "permute_backward_kernel launch");
+           "unpermute_kernel launch");
   return MOE_OK;
 }
 
 int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, const void* y, int y_dtype,
-                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const float* topk_w,
-                         int64_t T, int k, int64_t E, int64_t H, void* dy, float* dw, int32_t* status,
+                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const void* w, int w_dtype,
+                         int64_t T, int k, int64_t E, int64_t H, void* dy, void* dw, int32_t* status,
                          void* stream) {
   int sms = 0;
   int rc = device_info(&sms);
@@ -1595,7 +1604,8 @@ int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, 
   if (!rc && dw) rc = check_rows("y", y, y_dtype, y_stride, H);
   if (!rc && dy) rc = check_rows("dy", dy, y_dtype, H, H);
   if (rc) return rc;
-  CHECK_ARG(pos && offsets && topk_w && E >= 1, "null grouping");
+  CHECK_ARG(pos && offsets && w && E >= 1, "null grouping");
+  CHECK_ARG(is_float(w_dtype), "weights: dtype must be bf16, f16 or f32");
   moe::permute::Params p{};
   p.x = dout;
   p.x_dt = dout_dtype;
@@ -1607,7 +1617,8 @@ int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, 
   p.out_dt = y_dtype;
   p.pos = pos;
   p.n_rows = offsets + E;
-  p.w = topk_w;
+  p.w = w;
+  p.w_dt = w_dtype;
   p.dw = dw;
   p.status = status;
   p.T = T;
@@ -1631,43 +1642,105 @@ constexpr int64_t kNormMaxSlabs = 592;
 
 struct NormShape {
   int threads, rows_per_cta;
-  NormKernel forward, backward;
+  NormKernel kernel;
 };
 
-template <int kTpr, int kNv>
-NormShape norm_shape(bool vec) {
+template <class T, int kTpr, int kNv, bool kVec>
+NormShape norm_forward_shape() {
   using G = moe::norm::Group<kTpr>;
-  NormShape s;
-  s.threads = G::kThreads;
-  s.rows_per_cta = G::kRpc;
-  s.forward = vec ? moe::norm::norm_forward_kernel<kTpr, kNv, true> : moe::norm::norm_forward_kernel<kTpr, kNv, false>;
-  s.backward =
-      vec ? moe::norm::norm_backward_kernel<kTpr, kNv, true> : moe::norm::norm_backward_kernel<kTpr, kNv, false>;
-  return s;
+  return {G::kThreads, G::kRpc, moe::norm::norm_forward_kernel<T, kTpr, kNv, kVec>};
 }
 
-// Threads per row: the fewest of 32, 64, ... that hold H at 8 values each.
-NormShape norm_shape_for(int64_t H, bool vec) {
-  const int64_t v = (H + 7) / 8;
-  if (v <= 32) return norm_shape<32, 1>(vec);
-  if (v <= 64) return norm_shape<64, 1>(vec);
-  if (v <= 128) return norm_shape<128, 1>(vec);
-  if (v <= 256) return norm_shape<256, 1>(vec);
-  if (v <= 512) return norm_shape<512, 1>(vec);
-  if (v <= 1024) return norm_shape<1024, 1>(vec);
-  return norm_shape<1024, 2>(vec);
+// One vector (8 values) per thread and any types: the shortest time for one
+// row, and the only form for rows without 16-byte accesses or for mixed types.
+template <bool kVec>
+NormShape norm_forward_any(int64_t v) {
+  using T = moe::norm::AnyTypes;
+  if (v <= 32) return norm_forward_shape<T, 32, 1, kVec>();
+  if (v <= 64) return norm_forward_shape<T, 64, 1, kVec>();
+  if (v <= 128) return norm_forward_shape<T, 128, 1, kVec>();
+  if (v <= 256) return norm_forward_shape<T, 256, 1, kVec>();
+  if (v <= 512) return norm_forward_shape<T, 512, 1, kVec>();
+  if (v <= 1024) return norm_forward_shape<T, 1024, 1, kVec>();
+  return norm_forward_shape<T, 1024, 2, kVec>();
 }
 
-int norm_rows_per_cta(int64_t H) {
-  const int64_t v = (H + 7) / 8;
-  return v <= 32 ? 8 : v <= 64 ? 4 : v <= 128 ? 2 : 1;
+// Two vectors per thread and fixed types, once there are rows enough for every
+// SM: half the warps to join in each sum and twice the loads in flight.
+template <class T>
+NormShape norm_forward_fixed(int64_t v) {
+  if (v <= 64) return norm_forward_shape<T, 32, 2, true>();
+  if (v <= 128) return norm_forward_shape<T, 64, 2, true>();
+  if (v <= 256) return norm_forward_shape<T, 128, 2, true>();
+  if (v <= 512) return norm_forward_shape<T, 256, 2, true>();
+  return norm_forward_shape<T, 512, 2, true>();
 }
 
-int64_t norm_slabs(int64_t T, int64_t H) {
-  const int64_t rpc = norm_rows_per_cta(H);
-  const int64_t ctas = (T + rpc - 1) / rpc;
-  return ctas < kNormMaxSlabs ? ctas : kNormMaxSlabs;
+template <int kTpr, int kNv, bool kVec>
+NormShape norm_backward_shape() {
+  using G = moe::norm::Group<kTpr>;
+  return {G::kThreads, G::kRpc, moe::norm::norm_backward_kernel<kTpr, kNv, kVec>};
 }
+
+template <bool kVec>
+NormShape norm_backward_any(int64_t v) {
+  if (v <= 32) return norm_backward_shape<32, 1, kVec>();
+  if (v <= 64) return norm_backward_shape<64, 1, kVec>();
+  if (v <= 128) return norm_backward_shape<128, 1, kVec>();
+  if (v <= 256) return norm_backward_shape<256, 1, kVec>();
+  if (v <= 512) return norm_backward_shape<512, 1, kVec>();
+  return v <= 1024 ? norm_backward_shape<1024, 1, kVec>() : norm_backward_shape<1024, 2, kVec>();
+}
+
+constexpr int kRingSmem = 216 * 1024;
+using RingKernel = void (*)(const moe::norm::RingParams);
+struct RingShape {
+  int threads, rows_per_cta, columns;  // columns: a row's slot in a stage
+  RingKernel kernel;
+};
+
+template <class T, int kTpr>
+RingShape ring_shape() {
+  using G = moe::norm::RingGroup<kTpr>;
+  // once per kernel and process: the largest ring that it may be given
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(moe::norm::norm_backward_ring_kernel<T, kTpr, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         kRingSmem);
+  });
+  return {G::kThreads, G::kRpc, kTpr * 16, moe::norm::norm_backward_ring_kernel<T, kTpr, 2>};
+}
+
+template <class T>
+RingShape norm_backward_ring(int64_t v) {
+  if (v <= 64) return ring_shape<T, 32>();
+  if (v <= 128) return ring_shape<T, 64>();
+  if (v <= 256) return ring_shape<T, 128>();
+  if (v <= 512) return ring_shape<T, 256>();
+  return ring_shape<T, 512>();
+}
+
+// The kernels with fixed types: `f(Types)` for the combination of one call, if
+// it is one of them (all 16-bit or all f32 with the weights in that type or
+// f32, or a bf16 branch on an f32 residual stream); false otherwise.
+template <typename F>
+bool norm_fixed_types(const MoeNormDesc* d, bool has_y, bool has_post, bool has_next, F&& f) {
+  constexpr int kB = MOE_DT_BF16, kH = MOE_DT_F16, kF = MOE_DT_F32;
+  const int res = d->res_dtype, y = has_y ? d->y_dtype : has_next ? d->norm_dtype : res;
+  const int norm = has_next ? d->norm_dtype : y;
+  const int w = has_next ? d->next_dtype : has_post ? d->post_dtype : kF;
+  if ((has_post && d->post_dtype != w) || (d->gate_mode != MOE_GATE_NONE && d->gate_dtype != y) || norm != y)
+    return false;
+  if (res == kB && y == kB && w == kB) { f(moe::norm::Types<kB, kB, kB, kB>{}); return true; }
+  if (res == kB && y == kB && w == kF) { f(moe::norm::Types<kB, kB, kB, kF>{}); return true; }
+  if (res == kH && y == kH && w == kH) { f(moe::norm::Types<kH, kH, kH, kH>{}); return true; }
+  if (res == kH && y == kH && w == kF) { f(moe::norm::Types<kH, kH, kH, kF>{}); return true; }
+  if (res == kF && y == kF && w == kF) { f(moe::norm::Types<kF, kF, kF, kF>{}); return true; }
+  if (res == kF && y == kB && w == kF) { f(moe::norm::Types<kB, kF, kB, kF>{}); return true; }
+  return false;
+}
+
+int64_t norm_slabs(int64_t T) { return T < kNormMaxSlabs ? T : kNormMaxSlabs; }
 
 int norm_params(const MoeNormDesc* d, const void* y, const void* residual, const void* post, const void* next,
                 const void* gate, moe::norm::Params* p, bool* vec) {
@@ -1731,9 +1804,12 @@ int moe_norm_gate_residual(const MoeNormDesc* d, const void* y, const void* resi
   p.out = out;
   p.normed = normed;
   vec = vec && aligned16(out) && aligned16(normed);
-  const NormShape s = norm_shape_for(d->H, vec);
+  const int64_t v = (d->H + 7) / 8;
+  NormShape s = vec ? norm_forward_any<true>(v) : norm_forward_any<false>(v);
+  if (vec && v <= 1024 && d->T > 2 * sms)
+    norm_fixed_types(d, y, post_weight, next_weight, [&](auto types) { s = norm_forward_fixed<decltype(types)>(v); });
   const int64_t grid = (d->T + s.rows_per_cta - 1) / s.rows_per_cta;
-  CUDA_TRY(launch_pdl(s.forward, dim3(static_cast<unsigned>(grid)), dim3(s.threads), 0,
+  CUDA_TRY(launch_pdl(s.kernel, dim3(static_cast<unsigned>(grid)), dim3(s.threads), 0,
                       static_cast<cudaStream_t>(stream), p),
            "norm_forward_kernel launch");
   return MOE_OK;
@@ -1741,14 +1817,15 @@ int moe_norm_gate_residual(const MoeNormDesc* d, const void* y, const void* resi
 
 size_t moe_norm_backward_workspace_bytes(int64_t T, int64_t H) {
   if (T <= 0 || H <= 0) return 0;
-  return static_cast<size_t>(norm_slabs(T, H)) * 3 * static_cast<size_t>(H) * sizeof(float);
+  return static_cast<size_t>(norm_slabs(T)) * 3 * static_cast<size_t>(H) * sizeof(float);
 }
 
 int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int64_t d_out_stride,
                                     const void* d_normed, int64_t d_normed_stride, const void* y,
                                     const void* residual, const void* post_weight, const void* next_weight,
                                     const void* gate, void* d_y, void* d_residual, void* d_post, void* d_next,
-                                    void* d_gate, void* workspace, size_t workspace_bytes, void* stream) {
+                                    void* d_gate, void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream) {
   int sms = 0;
   int rc = device_info(&sms);
   if (rc) return rc;
@@ -1787,10 +1864,60 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
   vec = vec && aligned16(d_out) && (!d_out || d_out_stride % 8 == 0) && aligned16(d_normed) &&
         (!d_normed || d_normed_stride % 8 == 0) && aligned16(d_y) && aligned16(d_residual) &&
         (d->gate_mode != MOE_GATE_FULL || aligned16(d_gate));
-  const NormShape sh = norm_shape_for(d->H, vec);
-  const int64_t grid = norm_slabs(d->T, d->H);
-  CUDA_TRY(launch_pdl(sh.backward, dim3(static_cast<unsigned>(grid)), dim3(sh.threads), 0, s, p),
-           "norm_backward_kernel launch");
+  // The ring where a stage of a CTA's rows fits beside the weights; a form without one otherwise.
+  const int64_t v = (d->H + 7) / 8;
+  moe::norm::RingParams rp{};
+  RingShape ring{};
+  if (vec && v <= 1024) {
+    const int64_t size[5] = {y ? int64_t(dt_size(d->y_dtype)) : 0, int64_t(dt_size(d->res_dtype)),
+                             d_out ? int64_t(dt_size(d->res_dtype)) : 0,
+                             d_normed ? int64_t(dt_size(d->norm_dtype)) : 0,
+                             d->gate_mode == MOE_GATE_FULL ? int64_t(dt_size(d->gate_dtype)) : 0};
+    norm_fixed_types(d, y, post_weight, next_weight, [&](auto types) { ring = norm_backward_ring<decltype(types)>(v); });
+    int64_t off = 0;
+    for (int i = 0; i < 5; ++i) {
+      rp.off[i] = static_cast<int>(off);
+      rp.row_bytes[i] = static_cast<int>(size[i] * d->H);
+      off += size[i] * ring.columns;
+    }
+    rp.stage_bytes = static_cast<int>(off);
+  }
+  int64_t grid = 0, cols = 0;
+  const int64_t stage_all = static_cast<int64_t>(rp.stage_bytes) * ring.rows_per_cta;
+  if (ring.kernel) {
+    const int64_t size[3] = {post_weight ? int64_t(dt_size(d->post_dtype)) : 0,
+                             next_weight ? int64_t(dt_size(d->next_dtype)) : 0,
+                             d->gate_mode == MOE_GATE_CHANNEL ? int64_t(dt_size(d->gate_dtype)) : 0};
+    for (int i = 0; i < 3; ++i) {
+      rp.col_bytes[i] = static_cast<int>(size[i] * d->H);
+      rp.col_slot[i] = static_cast<int>(size[i] * ring.columns);
+      cols += rp.col_slot[i];
+    }
+  }
+  if (ring.kernel && stage_all + cols <= kRingSmem) {
+    rp.p = p;
+    rp.status = status;
+    const int64_t fit = (kRingSmem - cols) / stage_all;
+    rp.stages = static_cast<int>(fit < moe::norm::kRingStages ? fit : moe::norm::kRingStages);
+    int64_t smem = rp.stages * stage_all;
+    for (int i = 0; i < 3; ++i) {
+      rp.col_off[i] = static_cast<int>(smem);
+      smem += rp.col_slot[i];
+    }
+    const int64_t join = ring.threads * 8 * int64_t(sizeof(float));
+    smem = smem > join ? smem : join;
+    grid = (d->T + ring.rows_per_cta - 1) / ring.rows_per_cta;
+    grid = grid < sms ? grid : sms;
+    CUDA_TRY(launch_pdl(ring.kernel, dim3(static_cast<unsigned>(grid)), dim3(ring.threads), static_cast<size_t>(smem),
+                        s, rp),
+             "norm_backward_ring_kernel launch");
+  } else {
+    const NormShape sh = vec ? norm_backward_any<true>(v) : norm_backward_any<false>(v);
+    grid = (d->T + sh.rows_per_cta - 1) / sh.rows_per_cta;
+    grid = grid < kNormMaxSlabs ? grid : kNormMaxSlabs;
+    CUDA_TRY(launch_pdl(sh.kernel, dim3(static_cast<unsigned>(grid)), dim3(sh.threads), 0, s, p),
+             "norm_backward_kernel launch");
+  }
   if (!sums) return MOE_OK;
   moe::norm::ReduceParams r;
   r.part = p.part;
@@ -1802,8 +1929,8 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
   r.dt[2] = d->gate_dtype;
   r.slabs = static_cast<int>(grid);
   r.H = static_cast<int>(d->H);
-  CUDA_TRY(launch_pdl(moe::norm::norm_reduce_kernel, dim3(static_cast<unsigned>((d->H + 31) / 32), 3), dim3(256), 0,
-                      s, r),
+  CUDA_TRY(launch_pdl(moe::norm::norm_reduce_kernel, dim3(static_cast<unsigned>((d->H + 31) / 32), 3),
+                      dim3(moe::norm::kReduceThreads), 0, s, r),
            "norm_reduce_kernel launch");
   return MOE_OK;
 }

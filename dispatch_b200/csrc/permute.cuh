@@ -2,10 +2,11 @@
 // grouped row of flat slot f = t k + s (grouping.py; -1: the slot has no row):
 //
 //   permute            xs[pos[f]] = x[t]
-//   permute backward   dx[t]      = sum_s dxs[pos[f]]
+//   unpermute          out[t]     = sum_s w[f] rows[pos[f]] (+ shared[t])
+//                      (the combine; with w = 1 the gradient of permute)
 //   combine backward   dy[pos[f]] = w[f] dout[t],   dw[f] = <dout[t], y[pos[f]]>
 //
-// (the combine itself is combine.cuh). All three are bound by HBM: a token's
+// All three are bound by HBM: a token's
 // row is read or written once and its k grouped rows once. A CTA takes one
 // token and 8 columns per thread and step, so the k rows' loads or stores of a
 // step are in flight together. Every output element has one writer; sums run
@@ -15,6 +16,7 @@
 // of a product over all rows.
 #pragma once
 #include "combine.cuh"
+#include "norm.cuh"
 
 namespace moe {
 namespace permute {
@@ -24,19 +26,19 @@ constexpr int kMaxK = combine::kMaxK;
 constexpr int kSlots = 8;  // slots handled together in the combine backward
 
 struct Params {
-  const void* x;     // (T, H): x, or dout
-  const void* rows;  // (T*k, H): dxs, or y (combine backward; null without dw)
+  const void* x;     // (T, H): x, dout, or the shared rows
+  const void* rows;  // (T*k, H): the rows summed, or y (combine backward; unused without dw)
   void* out_rows;    // (T*k, H): xs, or dy
-  void* out;         // (T, H): dx
+  void* out;         // (T, H)
   const int32_t* pos;
-  const float* w;
-  float* dw;
+  const void* w;     // (T*k) in w_dt
+  void* dw;
   const int32_t* n_rows;  // offsets + E: rows in use
   int32_t* status;
   int64_t T, H;
   int64_t x_stride, rows_stride;  // elements between rows
   int k;
-  int x_dt, rows_dt, out_dt;  // out_dt: dx, or dy
+  int x_dt, rows_dt, out_dt, w_dt;  // out_dt: out, or dy
 };
 
 // Grouped row of slot f, or -1; a corrupted position raises the status.
@@ -86,22 +88,31 @@ __global__ void __launch_bounds__(kMaxThreads) permute_kernel(const Params p) {
 }
 
 // One CTA per token: the slots' rows of 8 columns, summed in slot order.
-__global__ void __launch_bounds__(kMaxThreads) permute_backward_kernel(const Params p) {
+// kWeighted: times w.
+template <bool kWeighted>
+__global__ void __launch_bounds__(kMaxThreads) unpermute_kernel(const Params p) {
   pdl_trigger();
   pdl_wait();  // before the first global memory access
   __shared__ int row[kMaxK];
+  __shared__ float weight[kMaxK];
   const int64_t t = blockIdx.x;
-  if (threadIdx.x < p.k) row[threadIdx.x] = row_of(p, t * p.k + threadIdx.x);
+  if (threadIdx.x < p.k) {
+    row[threadIdx.x] = row_of(p, t * p.k + threadIdx.x);
+    if (kWeighted) weight[threadIdx.x] = norm::load_one(p.w, p.w_dt, t * p.k + threadIdx.x);
+  }
   __syncthreads();
   for (int64_t h = threadIdx.x * 8; h < p.H; h += blockDim.x * 8) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto add = [&](int s, const float (&v)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = kWeighted ? fmaf(weight[s], v[i], acc[i]) : acc[i] + v[i];
+    };
     if (p.rows_dt == MOE_DT_F32) {
       for (int s = 0; s < p.k; ++s) {
         if (row[s] < 0) continue;
         float v[8];
         combine::load8(p.rows, p.rows_dt, row[s] * p.rows_stride + h, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += v[i];
+        add(s, v);
       }
     } else {
       for (int s0 = 0; s0 < p.k; s0 += kSlots) {
@@ -114,12 +125,18 @@ __global__ void __launch_bounds__(kMaxThreads) permute_backward_kernel(const Par
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
           if (s0 + j >= p.k) break;
+          if (row[s0 + j] < 0) continue;
           float v[8];
           combine::unpack8(raw[j], p.rows_dt, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] += v[i];
+          add(s0 + j, v);
         }
       }
+    }
+    if (p.x) {
+      float v[8];
+      combine::load8(p.x, p.x_dt, t * p.x_stride + h, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += v[i];
     }
     combine::store8(p.out, p.out_dt, t * p.H + h, acc);
   }
@@ -137,7 +154,7 @@ __global__ void __launch_bounds__(kMaxThreads) combine_backward_kernel(const Par
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < p.k) {
     row[threadIdx.x] = row_of(p, t * p.k + threadIdx.x);
-    weight[threadIdx.x] = p.w[t * p.k + threadIdx.x];
+    weight[threadIdx.x] = norm::load_one(p.w, p.w_dt, t * p.k + threadIdx.x);
   }
   __syncthreads();
   for (int s0 = 0; s0 < p.k; s0 += kSlots) {
@@ -188,7 +205,7 @@ __global__ void __launch_bounds__(kMaxThreads) combine_backward_kernel(const Par
     if (threadIdx.x < p.k) {
       float s = 0.f;
       for (int w = 0; w < static_cast<int>(blockDim.x / 32); ++w) s += sums[w][threadIdx.x];
-      p.dw[t * p.k + threadIdx.x] = s;  // a slot without a row contributes nothing: 0
+      norm::store_one(p.dw, p.w_dt, t * p.k + threadIdx.x, s);  // a slot without a row contributes nothing: 0
     }
   }
   if (p.out_rows) zero_tail(p, p.out_rows, p.out_dt == MOE_DT_F32 ? 4 : 2);

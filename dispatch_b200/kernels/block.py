@@ -22,14 +22,12 @@ from dispatch_b200 import _lib as L
 def _rows(t: torch.Tensor, h: int) -> tuple[torch.Tensor, int]:
     """``t`` (..., h) as rows with unit last stride, and their stride; copied
     only if its rows do not lie at one stride of at least h."""
-    r = t.reshape(-1, h)
-    if r.stride(1) != 1 and h > 1:
+    if t.is_contiguous():
+        return t, h
+    r = t.detach().reshape(-1, h)
+    if (r.stride(1) != 1 and h > 1) or (r.shape[0] > 1 and r.stride(0) < h):
         r = r.contiguous()
-    if r.shape[0] <= 1:
-        return r, h
-    if r.stride(0) < h:
-        r = r.contiguous()
-    return r, r.stride(0)
+    return r, r.stride(0) if r.shape[0] > 1 else h
 
 
 def _gate_mode(gate: torch.Tensor | None, y: torch.Tensor) -> int:
@@ -45,90 +43,86 @@ def _gate_mode(gate: torch.Tensor | None, y: torch.Tensor) -> int:
                      f"{tuple(y.shape)}")
 
 
-class _Call:
-    """Checked arguments of one call, as the C ABI takes them."""
-
-    def __init__(self, what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype, *grads):
-        self.dev = L.require_cuda(y, residual, post_weight, next_weight, gate, *grads, what=what)
-        if residual.dim() < 1 or residual.shape[-1] < 1:
-            raise ValueError(f"{what}: expected (..., H) with H >= 1, got {tuple(residual.shape)}")
-        if y is not None and y.shape != residual.shape:
-            raise ValueError(f"{what}: y.shape {tuple(y.shape)} != residual.shape {tuple(residual.shape)}")
-        self.shape, h = residual.shape, residual.shape[-1]
-        for name, w in (("post_weight", post_weight), ("next_weight", next_weight)):
-            if w is not None and w.shape != (h,):
-                raise ValueError(f"{what}: {name}.shape {tuple(w.shape)} != ({h},)")
-        if y is None and next_weight is None:
+def _describe(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype, *grads):
+    """The device, the descriptor and the (kept alive) inputs of one call, all
+    checked, as the C ABI takes them."""
+    dev = L.require_cuda(y, residual, post_weight, next_weight, gate, *grads, what=what)
+    shape = residual.shape
+    h = shape[-1] if len(shape) else 0
+    if h < 1:
+        raise ValueError(f"{what}: expected (..., H) with H >= 1, got {tuple(shape)}")
+    if y is None:
+        if next_weight is None:
             raise ValueError(f"{what}: nothing to compute without y and next_weight")
-        mode = _gate_mode(gate, residual)
-        d = self.desc = L.MoeNormDesc()
-        self.residual, d.res_stride = _rows(residual.detach(), h)
-        d.T, d.H = self.residual.shape
-        self.y = self.gate = None
-        if y is not None:
-            self.y, d.y_stride = _rows(y.detach(), h)
-            d.y_dtype = L.dt(y)
-        if gate is not None:
-            d.gate_dtype = L.dt(gate)
-            if mode == L.GATE_FULL:
-                self.gate, d.gate_stride = _rows(gate.detach(), h)
-            elif mode == L.GATE_TOKEN:
-                self.gate = gate.detach().reshape(-1, 1)
-                d.gate_stride = self.gate.stride(0)
-            else:
-                self.gate = gate.detach().contiguous()
+    elif y.shape != shape:
+        raise ValueError(f"{what}: y.shape {tuple(y.shape)} != residual.shape {tuple(shape)}")
+    for name, w in (("post_weight", post_weight), ("next_weight", next_weight)):
+        if w is not None and w.shape != (h,):
+            raise ValueError(f"{what}: {name}.shape {tuple(w.shape)} != ({h},)")
+    mode = _gate_mode(gate, residual)
+    d = L.MoeNormDesc()
+    d.T, d.H = residual.numel() // h, h
+    residual, d.res_stride = _rows(residual, h)
+    d.res_dtype = L.dt(residual)
+    if y is not None:
+        y, d.y_stride = _rows(y, h)
+        d.y_dtype = L.dt(y)
+    if gate is not None:
+        d.gate_dtype = L.dt(gate)
+        if mode == L.GATE_FULL:
+            gate, d.gate_stride = _rows(gate, h)
+        elif mode == L.GATE_TOKEN:
+            gate = gate.detach().reshape(-1, 1)
+            d.gate_stride = gate.stride(0)
+        else:
+            gate = gate.contiguous()
         d.gate_mode = mode
-        d.res_dtype = L.dt(residual)
-        self.post = None if post_weight is None else post_weight.detach().contiguous()
-        self.next = None if next_weight is None else next_weight.detach().contiguous()
-        d.post_dtype = 0 if post_weight is None else L.dt(post_weight)
-        d.next_dtype = 0 if next_weight is None else L.dt(next_weight)
-        self.norm_dtype = norm_dtype or residual.dtype
-        d.norm_dtype = L.dt(self.norm_dtype)
-        d.residual_scale, d.eps = float(residual_scale), float(eps)
-
-    def inputs(self):
-        return L.ptr(self.y), self.residual.data_ptr(), L.ptr(self.post), L.ptr(self.next), L.ptr(self.gate)
+    if post_weight is not None:
+        post_weight = post_weight.contiguous()
+        d.post_dtype = L.dt(post_weight)
+    if next_weight is not None:
+        next_weight = next_weight.contiguous()
+        d.next_dtype = L.dt(next_weight)
+    d.norm_dtype = d.res_dtype if norm_dtype is None else L.dt(norm_dtype)
+    d.residual_scale, d.eps = residual_scale, eps
+    return dev, d, (y, residual, post_weight, next_weight, gate)
 
 
 def _forward(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype):
-    c = _Call(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype)
-    out = torch.empty(c.shape, dtype=residual.dtype, device=c.dev) if y is not None else None
-    normed = torch.empty(c.shape, dtype=c.norm_dtype, device=c.dev) if next_weight is not None else None
-    with L.device_guard(c.dev):
-        rc = L.lib().moe_norm_gate_residual(ctypes.byref(c.desc), *c.inputs(), L.ptr(out), L.ptr(normed),
-                                            L.stream_ptr(c.dev))
-    L.check(rc, what)
+    dev, d, inputs = _describe(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype)
+    shape = residual.shape
+    out = torch.empty(shape, dtype=residual.dtype, device=dev) if y is not None else None
+    normed = torch.empty(shape, dtype=norm_dtype or residual.dtype, device=dev) if next_weight is not None else None
+    L.call(what, dev, L.lib().moe_norm_gate_residual, ctypes.byref(d), *map(L.ptr, inputs), L.ptr(out),
+           L.ptr(normed), L.stream_ptr(dev))
     return out, normed
 
 
 def _backward(what, d_out, d_normed, y, residual, post_weight, next_weight, gate, residual_scale, eps, needs):
-    norm_dtype = residual.dtype if d_normed is None else d_normed.dtype
-    c = _Call(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype, d_out, d_normed)
-    h = c.shape[-1]
+    norm_dtype = None if d_normed is None else d_normed.dtype
+    dev, d, inputs = _describe(what, y, residual, post_weight, next_weight, gate, residual_scale, eps, norm_dtype,
+                               d_out, d_normed)
+    shape, h = residual.shape, residual.shape[-1]
     for name, g in (("d_out", d_out), ("d_normed", d_normed)):
-        if g is not None and g.shape != c.shape:
-            raise ValueError(f"{what}: {name}.shape {tuple(g.shape)} != {tuple(c.shape)}")
-    if d_normed is not None and next_weight is None:
-        raise ValueError(f"{what}: d_normed needs next_weight")
+        if g is not None and g.shape != shape:
+            raise ValueError(f"{what}: {name}.shape {tuple(g.shape)} != {tuple(shape)}")
     s_out = s_normed = h
     if d_out is not None:
-        d_out, s_out = _rows(d_out.detach().to(residual.dtype), h)
+        d_out, s_out = _rows(d_out if d_out.dtype == residual.dtype else d_out.detach().to(residual.dtype), h)
     if d_normed is not None:
-        d_normed, s_normed = _rows(d_normed.detach(), h)
-    like = (y, residual, post_weight, next_weight, gate)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=c.dev) if t is not None and n else None
-             for t, n in zip(like, needs)]
-    ws = None
-    if grads[2] is not None or grads[3] is not None or (grads[4] is not None and c.desc.gate_mode == L.GATE_CHANNEL):
+        if next_weight is None:
+            raise ValueError(f"{what}: d_normed needs next_weight")
+        d_normed, s_normed = _rows(d_normed, h)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None and n else None
+             for t, n in zip((y, residual, post_weight, next_weight, gate), needs)]
+    lib, ws, nbytes = L.lib(), None, 0
+    if grads[2] is not None or grads[3] is not None or (grads[4] is not None and d.gate_mode == L.GATE_CHANNEL):
         # per call, not cached: a captured graph then owns the workspace it replays on
-        ws = torch.empty(L.lib().moe_norm_backward_workspace_bytes(c.desc.T, h), dtype=torch.uint8, device=c.dev)
-    with L.device_guard(c.dev):
-        rc = L.lib().moe_norm_gate_residual_backward(
-            ctypes.byref(c.desc), L.ptr(d_out), s_out, L.ptr(d_normed), s_normed, *c.inputs(),
-            *(L.ptr(g) for g in grads), L.ptr(ws), 0 if ws is None else ws.numel(), L.stream_ptr(c.dev),
-        )
-    L.check(rc, what)
+        nbytes = lib.moe_norm_backward_workspace_bytes(d.T, h)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    L.call(what, dev, lib.moe_norm_gate_residual_backward, ctypes.byref(d), L.ptr(d_out), s_out, L.ptr(d_normed),
+           s_normed, *map(L.ptr, inputs), *map(L.ptr, grads), L.ptr(ws), nbytes, L.status_word(dev).data_ptr(),
+           L.stream_ptr(dev))
     return tuple(grads)
 
 

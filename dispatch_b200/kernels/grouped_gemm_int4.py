@@ -60,13 +60,12 @@ def grouped_matmul_int4(x: torch.Tensor, qweight: Int4Tensor, schedule: TileSche
     offsets = device_offsets(schedule, dev)
     lib = L.lib()
     ws = _workspace(lib.moe_int4_workspace_bytes(m, e, qweight.n, qweight.k), dev)
-    with L.device_guard(dev):
-        rc = lib.moe_grouped_gemm_int4(
-            x.data_ptr(), L.dt(x), m, qweight.k, qweight.data.data_ptr(), qweight.scale.data_ptr(),
-            L.dt(qweight.scale), qweight.group_size, e, qweight.n, offsets.data_ptr(), out.data_ptr(), qweight.n,
-            L.ptr(ws), 0 if ws is None else ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
-        )
-    L.check(rc, "grouped_matmul_int4")
+    L.call(
+        "grouped_matmul_int4", dev, lib.moe_grouped_gemm_int4,
+        x.data_ptr(), L.dt(x), m, qweight.k, qweight.data.data_ptr(), qweight.scale.data_ptr(),
+        L.dt(qweight.scale), qweight.group_size, e, qweight.n, offsets.data_ptr(), out.data_ptr(), qweight.n,
+        L.ptr(ws), 0 if ws is None else ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+    )
     return out
 
 
@@ -91,12 +90,11 @@ def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4Stacke
     y = torch.empty(r, h, dtype=xs.dtype, device=dev)
     lib = L.lib()
     ws = _workspace(lib.moe_ffn_int4_workspace_bytes(r, e, h, i), dev)
-    with L.device_guard(dev):
-        rc = lib.moe_expert_ffn_int4(
-            xs.data_ptr(), L.dt(xs), r, h, offsets.contiguous().data_ptr(), e, i, gate.data.data_ptr(),
-            gate.scale.data_ptr(), up.data.data_ptr(), up.scale.data_ptr(), down.data.data_ptr(),
-            down.scale.data_ptr(), L.dt(gate.scale), gate.group_size, y.data_ptr(), L.ptr(ws),
-            0 if ws is None else ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
-        )
-    L.check(rc, "expert_ffn_int4")
+    L.call(
+        "expert_ffn_int4", dev, lib.moe_expert_ffn_int4,
+        xs.data_ptr(), L.dt(xs), r, h, offsets.contiguous().data_ptr(), e, i, gate.data.data_ptr(),
+        gate.scale.data_ptr(), up.data.data_ptr(), up.scale.data_ptr(), down.data.data_ptr(),
+        down.scale.data_ptr(), L.dt(gate.scale), gate.group_size, y.data_ptr(), L.ptr(ws),
+        0 if ws is None else ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+    )
     return y

@@ -34,6 +34,35 @@ class TokenGrouping:
     top_k: int
 
 
+class _DeviceGrouping(TokenGrouping):
+    """A ``TokenGrouping`` whose int64 ``group_sizes`` and cast ``sorted_weight``
+    are made from the kernels' int32 counts and f32 weights when they are first
+    read: two launches that a caller who only permutes and combines never needs."""
+
+    @property
+    def group_sizes(self) -> torch.Tensor:
+        v = self.__dict__["_sizes"]
+        if v.dtype != torch.int64:
+            v = self.__dict__["_sizes"] = v.to(torch.int64)
+        return v
+
+    @group_sizes.setter
+    def group_sizes(self, value: torch.Tensor) -> None:
+        self.__dict__["_sizes"] = value
+
+    @property
+    def sorted_weight(self) -> torch.Tensor:
+        v, dtype = self.__dict__["_sorted"]
+        if v.dtype != dtype:
+            v = v.to(dtype)
+            self.__dict__["_sorted"] = v, dtype
+        return v
+
+    @sorted_weight.setter
+    def sorted_weight(self, value) -> None:
+        self.__dict__["_sorted"] = value if isinstance(value, tuple) else (value, value.dtype)
+
+
 def _group(topk_idx: torch.Tensor, topk_weight: torch.Tensor | None, n_experts: int,
            x: torch.Tensor | None = None, xs_dtype: torch.dtype | None = None,
            want_sorted: bool = True):
@@ -76,10 +105,12 @@ def group_tokens_by_expert(
             f"topk_idx.shape {tuple(topk_idx.shape)} != topk_weight.shape {tuple(topk_weight.shape)}"
         )
     counts, offsets, pos, sti, sw, w, _ = _group(topk_idx, topk_weight, n_routed_experts)
-    return TokenGrouping(
+    if torch.cuda.is_current_stream_capturing():  # part of the graph, or replays would not update them
+        counts, sw = counts.to(torch.int64), sw.to(topk_weight.dtype)
+    return _DeviceGrouping(
         sorted_token_idx=sti,
-        sorted_weight=sw.to(topk_weight.dtype),
-        group_sizes=counts.to(torch.int64),
+        sorted_weight=(sw, topk_weight.dtype),
+        group_sizes=counts,
         offsets=offsets,
         pos=pos,
         flat_weight=w.reshape(-1),
@@ -117,7 +148,7 @@ def ungroup_and_combine(
 
 
 # ---------------------------------------------------------------- with gradients
-def _check_grouping(what: str, grouping: TokenGrouping, rows: torch.Tensor | None, tokens: int | None) -> int:
+def _tokens(what: str, grouping: TokenGrouping, rows: torch.Tensor | None, tokens: int | None) -> int:
     """The token count of ``grouping``; raises if rows or tokens do not fit it."""
     n = grouping.pos.numel()
     t = n // grouping.top_k
@@ -128,61 +159,63 @@ def _check_grouping(what: str, grouping: TokenGrouping, rows: torch.Tensor | Non
     return t
 
 
-def _row_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (N, H), copied only if its rows cannot be read in 16-byte pieces
-    where they lie (a last stride other than 1, unaligned or overlapping rows)."""
+def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` (N, H) and its row stride, copied only if its rows cannot be read
+    in 16-byte pieces where they lie (a last stride other than 1, unaligned or
+    overlapping rows)."""
     if t.dim() != 2:
         raise ValueError(f"expected (rows, H), got {tuple(t.shape)}")
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    h = t.shape[1]
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t, h
+        if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= h:
+            return t, t.stride(0)
+    c = t.detach().contiguous()
+    return (c if c.data_ptr() % 16 == 0 else c.clone(memory_format=torch.contiguous_format)), h
 
 
-def _stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _flat_weight(what: str, topk_weight: torch.Tensor | None, grouping: TokenGrouping) -> torch.Tensor:
+def _weights(what: str, topk_weight: torch.Tensor | None, grouping: TokenGrouping) -> torch.Tensor:
+    """(T*k) weights in their own type."""
     if topk_weight is None:
         return grouping.flat_weight
     if topk_weight.numel() != grouping.pos.numel():
         raise ValueError(f"{what}: topk_weight has {topk_weight.numel()} values, grouping describes {grouping.pos.numel()}")
-    return topk_weight.detach().reshape(-1).float()
+    return topk_weight if topk_weight.is_contiguous() else topk_weight.detach().contiguous()
 
 
 def _permute(x: torch.Tensor, grouping: TokenGrouping) -> torch.Tensor:
     dev = L.require_cuda(x, grouping.pos, what="permute_tokens")
-    x = _row_view(x)
-    t = _check_grouping("permute_tokens", grouping, None, x.shape[0])
-    h = x.shape[1]
-    xs = torch.empty(t * grouping.top_k, h, dtype=x.dtype, device=dev)
-    with L.device_guard(dev):
-        rc = L.lib().moe_permute_rows(
-            x.data_ptr(), L.dt(x), _stride(x), grouping.pos.data_ptr(), grouping.offsets.data_ptr(), t,
-            grouping.top_k, grouping.offsets.numel() - 1, h, xs.data_ptr(), L.status_word(dev).data_ptr(),
-            L.stream_ptr(dev),
-        )
-    L.check(rc, "permute_tokens")
+    x, stride = _row_view(x)
+    t = _tokens("permute_tokens", grouping, None, x.shape[0])
+    h, k = x.shape[1], grouping.top_k
+    xs = torch.empty(t * k, h, dtype=x.dtype, device=dev)
+    L.call("permute_tokens", dev, L.lib().moe_permute_rows, x.data_ptr(), L.dt(x), stride, grouping.pos.data_ptr(),
+           grouping.offsets.data_ptr(), t, k, grouping.offsets.numel() - 1, h, xs.data_ptr(),
+           L.status_word(dev).data_ptr(), L.stream_ptr(dev))
     return xs
+
+
+def _unpermute(what, rows, grouping, w, y_shared, out_dtype) -> torch.Tensor:
+    dev = L.require_cuda(rows, grouping.pos, w, y_shared, what=what)
+    rows, stride = _row_view(rows)
+    t = _tokens(what, grouping, rows, None if y_shared is None else y_shared.shape[0])
+    h = rows.shape[1]
+    shared_stride = h
+    if y_shared is not None:
+        y_shared, shared_stride = _row_view(y_shared)
+    out = torch.empty(t, h, dtype=out_dtype or rows.dtype, device=dev)
+    L.call(what, dev, L.lib().moe_unpermute_rows, rows.data_ptr(), L.dt(rows), stride, grouping.pos.data_ptr(),
+           L.ptr(w), 0 if w is None else L.dt(w), L.ptr(y_shared), shared_stride, t, grouping.top_k, h,
+           out.data_ptr(), L.dt(out), L.status_word(dev).data_ptr(), L.stream_ptr(dev))
+    return out
 
 
 def permute_tokens_backward(dxs: torch.Tensor, grouping: TokenGrouping, *,
                             out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """dx[t] = sum over the token's slots of dxs[pos], in f32 in slot order,
     rounded once to ``out_dtype`` (default: dxs' type)."""
-    dev = L.require_cuda(dxs, grouping.pos, what="permute_tokens_backward")
-    dxs = _row_view(dxs)
-    t = _check_grouping("permute_tokens_backward", grouping, dxs, None)
-    h = dxs.shape[1]
-    dx = torch.empty(t, h, dtype=out_dtype or dxs.dtype, device=dev)
-    with L.device_guard(dev):
-        rc = L.lib().moe_permute_rows_backward(
-            dxs.data_ptr(), L.dt(dxs), _stride(dxs), grouping.pos.data_ptr(), t, grouping.top_k, h, dx.data_ptr(),
-            L.dt(dx), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
-        )
-    L.check(rc, "permute_tokens_backward")
-    return dx
+    return _unpermute("permute_tokens_backward", dxs, grouping, None, None, out_dtype)
 
 
 class _Permute(torch.autograd.Function):
@@ -208,16 +241,12 @@ def permute_tokens(x: torch.Tensor, grouping: TokenGrouping) -> torch.Tensor:
 
 
 def _combine(y, grouping, topk_weight, y_shared, out_dtype) -> torch.Tensor:
-    dev = L.require_cuda(y, grouping.pos, topk_weight, y_shared, what="combine_tokens")
-    t = _check_grouping("combine_tokens", grouping, y, None if y_shared is None else y_shared.shape[0])
-    w = _flat_weight("combine_tokens", topk_weight, grouping)
+    w = _weights("combine_tokens", topk_weight, grouping)
     if y_shared is not None and y_shared.dtype != y.dtype:
         raise ValueError(f"dtype mismatch: y is {y.dtype}, y_shared is {y_shared.dtype}")
     if y_shared is not None and y_shared.shape[1:] != y.shape[1:]:
         raise ValueError(f"y_shared.shape {tuple(y_shared.shape)} does not match rows of {tuple(y.shape)}")
-    with L.device_guard(dev):
-        return combine(y.detach(), grouping.pos, w, t, grouping.top_k,
-                       None if y_shared is None else y_shared.detach(), out_dtype)
+    return _unpermute("combine_tokens", y, grouping, w, y_shared, out_dtype)
 
 
 def combine_tokens_backward(
@@ -225,27 +254,26 @@ def combine_tokens_backward(
     need_y: bool = True, need_weight: bool = True,
 ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """The gradients (dy, dweight) of ``combine_tokens``: dy[pos[f]] = w[f] *
-    dout[f/k] in y's type, zero in rows that no slot owns; dweight (T, k) =
-    <dout[f/k], y[pos[f]]>, summed in f32, in topk_weight's type (f32 for the
-    grouping's own weights). y_shared's gradient is dout itself."""
-    dev = L.require_cuda(dout, y, grouping.pos, topk_weight, what="combine_tokens_backward")
-    y, dout = _row_view(y), _row_view(dout)
-    t = _check_grouping("combine_tokens_backward", grouping, y, dout.shape[0])
-    if dout.shape[1] != y.shape[1]:
-        raise ValueError(f"dout.shape {tuple(dout.shape)} does not match rows of {tuple(y.shape)}")
-    w = _flat_weight("combine_tokens_backward", topk_weight, grouping)
+    dout[f/k] in y's type, zero in rows that no slot owns; dweight =
+    <dout[f/k], y[pos[f]]>, summed in f32, in topk_weight's type and shape
+    ((T, k) f32 for the grouping's own weights). y_shared's gradient is dout
+    itself."""
+    what = "combine_tokens_backward"
+    dev = L.require_cuda(dout, y, grouping.pos, topk_weight, what=what)
+    y, y_stride = _row_view(y)
+    dout, dout_stride = _row_view(dout)
+    t = _tokens(what, grouping, y, dout.shape[0])
     h, k = y.shape[1], grouping.top_k
-    dy = torch.empty(y.shape[0], h, dtype=y.dtype, device=dev) if need_y else None
-    dw = torch.empty(t, k, dtype=torch.float32, device=dev) if need_weight else None
-    with L.device_guard(dev):
-        rc = L.lib().moe_combine_backward(
-            dout.data_ptr(), L.dt(dout), _stride(dout), y.data_ptr(), L.dt(y), _stride(y), grouping.pos.data_ptr(),
-            grouping.offsets.data_ptr(), w.data_ptr(), t, k, grouping.offsets.numel() - 1, h, L.ptr(dy), L.ptr(dw),
-            L.status_word(dev).data_ptr(), L.stream_ptr(dev),
-        )
-    L.check(rc, "combine_tokens_backward")
-    if dw is not None and topk_weight is not None:
-        dw = dw.to(topk_weight.dtype).view(topk_weight.shape)
+    if dout.shape[1] != h:
+        raise ValueError(f"dout.shape {tuple(dout.shape)} does not match rows of {tuple(y.shape)}")
+    w = _weights(what, topk_weight, grouping)
+    dy = torch.empty(t * k, h, dtype=y.dtype, device=dev) if need_y else None
+    dw = None
+    if need_weight:
+        dw = torch.empty((t, k) if topk_weight is None else topk_weight.shape, dtype=w.dtype, device=dev)
+    L.call(what, dev, L.lib().moe_combine_backward, dout.data_ptr(), L.dt(dout), dout_stride, y.data_ptr(), L.dt(y),
+           y_stride, grouping.pos.data_ptr(), grouping.offsets.data_ptr(), w.data_ptr(), L.dt(w), t, k,
+           grouping.offsets.numel() - 1, h, L.ptr(dy), L.ptr(dw), L.status_word(dev).data_ptr(), L.stream_ptr(dev))
     return dy, dw
 
 

@@ -186,13 +186,12 @@ def _expert_ffn_int4(xs, offsets, weights, shared: SharedExpertWeights | None, x
     ws = torch.empty(max(lib.moe_ffn_workspace_bytes(0, 0, t, i_sh), 256), dtype=torch.uint8, device=dev)
     x_shared = x_shared.contiguous()
     gate, up, down = shared.gate.contiguous(), shared.up.contiguous(), shared.down.contiguous()
-    with L.device_guard(dev):
-        rc = lib.moe_expert_ffn_grouped(
-            3, None, L.dt(act), 0, h, None, 1, 1, None, 0, 0, None, None, None, L.dt(act), None, None, None, 0,
-            x_shared.data_ptr(), t, i_sh, gate.data_ptr(), up.data_ptr(), down.data_ptr(), None, ys.data_ptr(),
-            ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
-        )
-    L.check(rc, "expert_ffn")
+    L.call(
+        "expert_ffn", dev, lib.moe_expert_ffn_grouped,
+        3, None, L.dt(act), 0, h, None, 1, 1, None, 0, 0, None, None, None, L.dt(act), None, None, None, 0,
+        x_shared.data_ptr(), t, i_sh, gate.data_ptr(), up.data_ptr(), down.data_ptr(), None, ys.data_ptr(),
+        ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
+    )
     return y, ys
 
 

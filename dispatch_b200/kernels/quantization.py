@@ -194,10 +194,8 @@ def quantize_groupwise_int4(weight: torch.Tensor, *, group_size: int = 128,
     e, n, k = w.shape
     data = torch.empty(e, -(-n // 16), -(-k // 64), 32, 4, dtype=torch.int32, device=dev)
     scale = torch.empty(e, -(-n // 16), -(-k // group_size), 16, dtype=scale_dtype, device=dev)
-    with L.device_guard(dev):
-        rc = L.lib().moe_quantize_int4(w.data_ptr(), L.dt(w), e, n, k, group_size, data.data_ptr(),
-                                       scale.data_ptr(), L.dt(scale), L.stream_ptr(dev))
-    L.check(rc, "quantize_groupwise_int4")
+    L.call("quantize_groupwise_int4", dev, L.lib().moe_quantize_int4, w.data_ptr(), L.dt(w), e, n, k, group_size,
+           data.data_ptr(), scale.data_ptr(), L.dt(scale), L.stream_ptr(dev))
     return Int4Tensor(data, scale, n, k, group_size)
 
 

@@ -305,24 +305,29 @@ int moe_layer_forward(const MoeLayerDesc* d, const void* x, const void* router_w
                       size_t workspace_bytes, int32_t* status, void* stream);
 
 /*
- * Row gather by a given grouping, and the gradients of the gather and of the
- * combine (the reference's grouping.py:25-61 is forward only). pos (T*k) and
+ * Row gather by a given grouping, the weighted sum back, and the combine's
+ * gradient (the reference's grouping.py:25-61 is forward only). pos (T*k) and
  * offsets (E+1) are moe_group_tokens' outputs; k <= 32, H a multiple of 8,
  * rows 16-byte aligned. Row strides are in elements (multiples of 8, >= H);
  * outputs are contiguous. A slot with pos = -1 has no row: it adds nothing
  * and its dw is 0. Rows at and after offsets[E] are written as zeros.
- *   moe_permute_rows           xs[pos[t*k+s]] = x[t]            (same type)
- *   moe_permute_rows_backward  dx[t] = sum_s dxs[pos[t*k+s]]    (slot order, f32, rounded once)
- *   moe_combine_backward       dy[pos[f]] = topk_w[f] * dout[f/k]   (y_dtype; dy NULL: skipped)
- *                              dw[f] = <dout[f/k], y[pos[f]]>       (f32; dw NULL: skipped, y may be NULL)
+ *   moe_permute_rows     xs[pos[t*k+s]] = x[t]             (same type)
+ *   moe_unpermute_rows   out[t] = sum_s w[t*k+s] * rows[pos[t*k+s]] (+ shared[t])
+ *                        in slot order in f32, rounded once: moe_combine with
+ *                        weights of any float type and strided rows. w NULL:
+ *                        all 1, the gradient of moe_permute_rows. shared
+ *                        (T, H) in the rows' type, may be NULL.
+ *   moe_combine_backward dy[pos[f]] = w[f] * dout[f/k]     (y_dtype; dy NULL: skipped)
+ *                        dw[f] = <dout[f/k], y[pos[f]]>    (w_dtype, summed in f32; dw NULL: skipped)
  */
 int moe_permute_rows(const void* x, int dtype, int64_t x_stride, const int32_t* pos, const int32_t* offsets,
                      int64_t T, int k, int64_t E, int64_t H, void* xs, int32_t* status, void* stream);
-int moe_permute_rows_backward(const void* dxs, int dxs_dtype, int64_t dxs_stride, const int32_t* pos, int64_t T,
-                              int k, int64_t H, void* dx, int dx_dtype, int32_t* status, void* stream);
+int moe_unpermute_rows(const void* rows, int rows_dtype, int64_t rows_stride, const int32_t* pos, const void* w,
+                       int w_dtype, const void* shared, int64_t shared_stride, int64_t T, int k, int64_t H,
+                       void* out, int out_dtype, int32_t* status, void* stream);
 int moe_combine_backward(const void* dout, int dout_dtype, int64_t dout_stride, const void* y, int y_dtype,
-                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const float* topk_w,
-                         int64_t T, int k, int64_t E, int64_t H, void* dy, float* dw, int32_t* status,
+                         int64_t y_stride, const int32_t* pos, const int32_t* offsets, const void* w, int w_dtype,
+                         int64_t T, int k, int64_t E, int64_t H, void* dy, void* dw, int32_t* status,
                          void* stream);
 
 /*
@@ -367,7 +372,8 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
                                     const void* d_normed, int64_t d_normed_stride, const void* y,
                                     const void* residual, const void* post_weight, const void* next_weight,
                                     const void* gate, void* d_y, void* d_residual, void* d_post, void* d_next,
-                                    void* d_gate, void* workspace, size_t workspace_bytes, void* stream);
+                                    void* d_gate, void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream);
 
 /*
  * Expert products with 4-bit weights and group scales (beside the int8 ones;
