@@ -126,12 +126,12 @@ _SIGNATURES = {
         [ctypes.POINTER(MoeNormDesc), _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p],
         _i32,
     ),
-    "moe_int4_workspace_bytes": ([_i64, _i64, _i64, _i64], _sz),
+    "moe_int4_workspace_bytes": ([_i64, _i64, _i64, _i64, _i32], _sz),
     "moe_grouped_gemm_int4": (
         [_p, _i32, _i64, _i64, _p, _p, _i32, _i32, _i64, _i64, _p, _p, _i64, _p, _sz, _p, _p],
         _i32,
     ),
-    "moe_ffn_int4_workspace_bytes": ([_i64, _i64, _i64, _i64], _sz),
+    "moe_ffn_int4_workspace_bytes": ([_i64, _i64, _i64, _i64, _i32], _sz),
     "moe_expert_ffn_int4": (
         [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _p, _sz, _p, _p],
         _i32,

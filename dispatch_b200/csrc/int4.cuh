@@ -17,9 +17,10 @@
 // a 64-column block (32 for groups of 32) is summed by the tensor cores in
 // f32 and then multiplied by its f32 scale: no weight is rounded.
 //
-// Few rows per expert: bound by the weights' bytes. See int4_kernel. Many
-// rows: the weights become 16-bit tiles in a workspace (dequant_kernel, one
-// rounding of code * scale to the activation type) for the tcgen05 kernels.
+// int4_kernel, here: a few rows per expert, warp-level MMAs. int4_tile_kernel,
+// int4_tile.cuh: more rows, tcgen05. Most rows: the weights become 16-bit tiles
+// in a workspace (dequant_kernel, one rounding of code * scale to the
+// activation type) for the 16-bit tcgen05 kernels.
 #pragma once
 #include "gemm_warp.cuh"
 #include "norm.cuh"
@@ -27,12 +28,12 @@
 namespace moe {
 namespace int4 {
 
-constexpr int kWarps = 8;           // consumer warps, one 64-column block of a stage each
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
 constexpr int kBlockBytes = 512;    // 16 rows x 64 columns
-constexpr int kTileStage = kWarps * kBlockBytes;  // a 16-row tile's bytes in a stage
 constexpr int kMaxE = 256;
-constexpr int kMaxStages = 16;
+constexpr int kMaxStages = 6;
+constexpr int kRanges = 8;          // K is summed as eight ranges of blocks, whatever the kernel's shape
 
 struct Params {
   const uint8_t* data0;  // laid out codes; data1: the up projection (SwiGLU)
@@ -48,38 +49,61 @@ struct Params {
   int n16, kb, groups;  // tiles of 16 rows, blocks of 64 columns, scale groups
   int group_shift;      // log2 of the group size
   int scale_dt, scale_shift;  // scale_shift: log2 of a scale's bytes
-  int f16, stages;
+  int chunk;            // blocks in a stage
+  int scale_slot;       // bytes of a tile's scales in a stage
+  int f32_slot;         // bytes of a tile's f32 scales of a stage (behind the ring: their copy for 16-bit scales)
+  int stage_bytes, stages;  // of one warp's ring
 };
 
-// The A operand of one MMA step from its word of eight codes.
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+  return r;
+}
+
+// The A operand of one MMA step from its word of eight codes u = code + 8,
+// exactly: a nibble under an exponent's mantissa is a float 2^m + u, from which
+// 2^m + 8 is subtracted.
 template <bool kF16>
 __device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4]) {
   if (kF16) {
-    // 1024 + u, and 1024 + 16 u for the nibble above it
-    const __half2 c0 = __float2half2_rn(1032.f), inv = __float2half2_rn(0.0625f), c1 = __float2half2_rn(-72.f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t v = w >> (8 * i);
-      const uint32_t lo = (v & 0x000F000Fu) | 0x64006400u, hi = (v & 0x00F000F0u) | 0x64006400u;
-      const __half2 l = __hsub2(*reinterpret_cast<const __half2*>(&lo), c0);
-      const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&hi), inv, c1);
-      a[2 * i] = *reinterpret_cast<const uint32_t*>(&l);
-      a[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h);
+      const uint32_t v = i ? w >> 8 : w;
+      const uint32_t lo = and_or(v, 0x000F000Fu, 0x64006400u);  // 1024 + u
+      const uint32_t hi = and_or(v, 0x00F000F0u, 0x64006400u);  // 1024 + 16 u
+      asm("sub.f16x2 %0, %1, %2;" : "=r"(a[2 * i]) : "r"(lo), "r"(0x64086408u));  // - 1032
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(a[2 * i + 1]) : "r"(hi), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
     }
   } else {
-    const __nv_bfloat162 c = __float2bfloat162_rn(136.f);  // 128 + u, less 136
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), c);
-      a[i] = *reinterpret_cast<const uint32_t*>(&d);
+      const uint32_t v = and_or(i ? w >> (4 * i) : w, 0x000F000Fu, 0x43004300u);  // 128 + u
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(a[i]) : "r"(v), "r"(0x3F803F80u), "r"(0xC308C308u));  // * 1 - 136
     }
   }
 }
 
+// D = A B + D, with a zero D at first. Not volatile: the compiler may interleave
+// the chains of several tiles and blocks.
+template <bool kF16, bool kFirst>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const float c0 = kFirst ? 0.f : d[0], c1 = kFirst ? 0.f : d[1], c2 = kFirst ? 0.f : d[2], c3 = kFirst ? 0.f : d[3];
+  if (kF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  }
+}
+
 struct Ctrl {
-  uint64_t full[kMaxStages];
-  uint64_t empty[kMaxStages];
+  uint64_t full[kWarps][kMaxStages];
   int abort;
   int experts;           // experts with rows
   int units;             // units of the launch (0 if the offsets are bad)
@@ -89,22 +113,16 @@ struct Ctrl {
 };
 constexpr uint32_t kCtrlBytes = (sizeof(Ctrl) + 127) & ~uint32_t(127);
 
-// A launch's shape: kMt 16-row weight tiles and kNt 8-row token tiles per unit.
-template <int kMt, int kNt>
-struct Shape {
-  static constexpr uint32_t kDataStage = kMt * kTileStage;
-  static constexpr uint32_t kRedBytes = kWarps * kMt * kNt * 4 * 32 * 4;
-  static constexpr int kTok = 8 * kNt;
+// Sums that wait in shared memory: kMt weight tiles x kNt token tiles of each warp.
+template <int kMt, int kNt, bool kSplit>
+struct Sums {
+  static constexpr uint32_t kBytes = kWarps * kMt * kNt * 4 * 32 * 4;
+  static constexpr uint32_t kBuffers = kSplit ? 2 : 1;  // read by other warps while the next unit's are made
+  static constexpr uint32_t kFixed = kCtrlBytes + kBuffers * kBytes;
 };
 
-__host__ __device__ inline uint32_t scale_stage_bytes(int mt, int group_shift, int scale_shift) {
-  return static_cast<uint32_t>(mt) * ((64 * kWarps) >> group_shift) * (16u << scale_shift);
-}
-
-template <int kMt, int kNt>
-__host__ __device__ constexpr uint32_t fixed_smem() {
-  return 128 + kCtrlBytes + 2 * Shape<kMt, kNt>::kRedBytes;
-}
+// Resident CTAs per SM that the kernel is built for.
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 // Where a unit lies.
 struct Unit {
@@ -112,42 +130,43 @@ struct Unit {
 };
 
 // A unit is kMt weight tiles (SwiGLU: half of them gate, half up rows) x one
-// token tile of one expert, over all of K; consecutive units walk an expert's
-// token tiles, then its weight tiles, so a CTA, which takes a contiguous run
-// of units, streams contiguous weights and finds its rows of x in L1. Warp 8
-// issues the bulk copies of 512-column stages (kMt tiles' blocks and their
-// scales) into a ring that runs on across units; each of the other eight
-// warps takes one 64-column block of a stage, so that one unit's columns are
-// spread over the CTA and even a single token's few units keep the whole GPU
-// loading. The warps' sums are joined in shared memory in a fixed order. A row's result
-// does not depend on the unit's shape or on the other rows.
-template <int kMt, int kNt, bool kSwiglu, bool kF16, bool kG32>
-__global__ void __launch_bounds__(kThreads, 2) int4_kernel(const Params p) {
-  using Sh = Shape<kMt, kNt>;
-  constexpr int kOutTiles = kSwiglu ? kMt / 2 : kMt;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  Ctrl& c = *reinterpret_cast<Ctrl*>(base);
-  float* red = reinterpret_cast<float*>(base + kCtrlBytes);
-  uint8_t* ring = base + kCtrlBytes + 2 * Sh::kRedBytes;
-  const uint32_t scale_stage = scale_stage_bytes(kMt, p.group_shift, p.scale_shift);
-  const uint32_t stage_bytes = Sh::kDataStage + scale_stage;
+// token tile of 8 kNt rows of one expert, over all of K. A CTA takes a
+// contiguous run of units; consecutive units walk an expert's token tiles,
+// then its weight tiles, so a CTA's warps find their rows of x in L1.
+//
+// Each warp streams weights for itself: its lane 0 brings `chunk` blocks of
+// codes and their scales per stage of the warp's own ring by bulk copies, and
+// nothing but the warp waits for them. kSplit false: a warp takes whole units,
+// and no warp ever waits for another. kSplit true (few units: one or two
+// decoded tokens): the eight warps share a unit, each one of the eight ranges
+// that K's blocks are split into. The ranges' sums are joined in order,
+// ((r0 + r1) + r2) + ..., in both forms, so a row's result depends neither on
+// the form nor on the tile sizes nor on the other rows.
+//
+// Bounded by issue: per 256 weights one MMA per token tile and 9 (f16) or 11
+// (bf16) instructions that make its operand.
+template <int kMt, int kNt, bool kSplit, bool kSwiglu, bool kF16, bool kG32>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(kNt)) int4_kernel(const __grid_constant__ Params p) {
+  constexpr int kOutMt = kSwiglu ? kMt / 2 : kMt;  // output tiles of a unit
+  constexpr int kTok = 8 * kNt;
+  using S = Sums<kMt, kNt, kSplit>;
+  extern __shared__ __align__(128) uint8_t int4_smem[];
+  Ctrl& c = *reinterpret_cast<Ctrl*>(int4_smem);
+  float* sums = reinterpret_cast<float*>(int4_smem + kCtrlBytes);
+  uint8_t* rings = int4_smem + kCtrlBytes + S::kBuffers * S::kBytes;
   volatile int* abort_flag = &c.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_trigger();
-  if (tid == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      mbar_init(&c.full[i], 1);
-      mbar_init(&c.empty[i], kWarps);
-    }
-    c.abort = 0;
+  if (tid < kWarps) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(&c.full[tid][i], 1);
+    if (tid == 0) c.abort = 0;
     fence_mbar_init();
   }
   pdl_wait();  // before the first global memory access
   for (int g = tid; g <= p.E; g += kThreads) c.off[g] = p.offsets[g];
   __syncthreads();
-  const int tile_units = (p.n16 + kOutTiles - 1) / kOutTiles;
+  const int tile_units = (p.n16 + kOutMt - 1) / kOutMt;
   if (warp == 0) {
     // the experts with rows and the units before each
     int n = 0, units = 0;
@@ -157,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) int4_kernel(const Params p) {
       const int rows = e < p.E ? c.off[e + 1] - c.off[e] : 0;
       bad |= rows < 0;
       const uint32_t has = __ballot_sync(0xffffffffu, rows > 0);
-      const int u = rows > 0 ? (rows + Sh::kTok - 1) / Sh::kTok * tile_units : 0;
+      const int u = rows > 0 ? (rows + kTok - 1) / kTok * tile_units : 0;
       int v = u;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -181,184 +200,308 @@ __global__ void __launch_bounds__(kThreads, 2) int4_kernel(const Params p) {
     }
   }
   __syncthreads();
-  const int u0 = static_cast<int>(static_cast<int64_t>(c.units) * blockIdx.x / gridDim.x);
   const int u1 = static_cast<int>(static_cast<int64_t>(c.units) * (blockIdx.x + 1) / gridDim.x);
-  if (u0 == u1) return;
-  int at = 0;  // index of the unit's expert
+  constexpr int kStep = kSplit ? 1 : kWarps;
+  const int u0 = static_cast<int>(static_cast<int64_t>(c.units) * blockIdx.x / gridDim.x) + (kSplit ? 0 : warp);
+  if (u0 >= u1) return;  // the whole warp, or (kSplit) the whole CTA
+  int at0 = 0;  // index of the first unit's expert
   {
     int hi = c.experts - 1;
-    while (at < hi) {
-      const int mid = (at + hi + 1) / 2;
-      if (c.first[mid] <= u0) at = mid; else hi = mid - 1;
+    while (at0 < hi) {
+      const int mid = (at0 + hi + 1) / 2;
+      if (c.first[mid] <= u0) at0 = mid; else hi = mid - 1;
     }
   }
-  auto locate = [&](int u) {
-    if (u >= c.first[at + 1]) ++at;
+  // unit u, at or after the last one located with `at`
+  auto locate = [&](int u, int& at) {
+    while (u >= c.first[at + 1]) ++at;
     Unit r;
     r.e = c.expert[at];
     const int begin = c.off[r.e], rows = c.off[r.e + 1] - begin;
-    const int tok_tiles = (rows + Sh::kTok - 1) / Sh::kTok;
-    const int local = u - c.first[at];
-    const int tile = local / tok_tiles, tok = local - tile * tok_tiles;
-    r.row0 = begin + tok * Sh::kTok;
-    r.rows = min(Sh::kTok, rows - tok * Sh::kTok);
-    r.tile0 = tile * kOutTiles;
+    int tile = u - c.first[at], tok = 0;
+    if (rows > kTok) {
+      const int tok_tiles = (rows + kTok - 1) / kTok;
+      tok = tile % tok_tiles;
+      tile /= tok_tiles;
+    }
+    r.row0 = begin + tok * kTok;
+    r.rows = min(kTok, rows - tok * kTok);
+    r.tile0 = tile * kOutMt;
     return r;
   };
-  const int stages_per_unit = (p.kb + kWarps - 1) / kWarps;
+  // this warp's blocks
+  const int range = (p.kb + kRanges - 1) / kRanges;
+  const int lo = kSplit ? min(p.kb, warp * range) : 0, hi = kSplit ? min(p.kb, lo + range) : p.kb;
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------ bulk copies
+  // ---------------------------------------------------------------- bulk copies (lane 0)
+  uint8_t* ring = rings + warp * (p.stages * p.stage_bytes + kMt * p.f32_slot);
+  float* f32_scales = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes);
+  int pu = u0, pb = lo, pat = at0;  // the next stage to bring: unit, first block
+  uint32_t pstage = 0;
+  int ptile = 0;            // first tile of the unit among all experts' ...
+  int ptiles = 0;           // ... and its tiles
+  auto place = [&]() {
+    const Unit r = locate(pu, pat);
+    ptile = r.e * p.n16 + r.tile0;
+    ptiles = min(kOutMt, p.n16 - r.tile0);
+  };
+  place();
+  if (lo == hi) pu = u1;  // K of fewer than eight blocks: nothing for this warp
+  auto issue = [&]() {
+    const int nb = min(p.chunk, hi - pb);
     if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      uint32_t issued_mask = 0, issued_parity = 0;
-      bool ok = true;
-      const uint32_t group_bytes = 16u << p.scale_shift;
-      for (int u = u0; ok && u < u1; ++u) {
-        const Unit r = locate(u);
-        const int tiles = min(kOutTiles, p.n16 - r.tile0);
-        for (int s = 0; s < stages_per_unit; ++s) {
-          if (!wait_parity_bounded(&c.empty[stage], phase ^ 1u, abort_flag, p.status)) { ok = false; break; }
-          const int b0 = s * kWarps, nb = min(kWarps, p.kb - b0);
-          const int g0 = (b0 * 64) >> p.group_shift;
-          const int ng = min((64 * kWarps) >> p.group_shift, p.groups - g0);
-          const uint32_t per_tile = nb * kBlockBytes + ng * group_bytes;
-          mbar_arrive_expect_tx(&c.full[stage], per_tile * tiles * (kSwiglu ? 2 : 1));
-          uint8_t* dst = ring + stage * stage_bytes;
-          for (int i = 0; i < (kSwiglu ? 2 : 1) * tiles; ++i) {
-            const bool up = kSwiglu && i >= tiles;
-            const int slot = up ? kOutTiles + i - tiles : i;
-            const int64_t tile = static_cast<int64_t>(r.e) * p.n16 + r.tile0 + (up ? i - tiles : i);
-            bulk_load(dst + slot * kTileStage, (up ? p.data1 : p.data0) + (tile * p.kb + b0) * kBlockBytes,
-                      nb * kBlockBytes, &c.full[stage]);
-            bulk_load(dst + Sh::kDataStage + slot * (scale_stage / kMt),
-                      (up ? p.scale1 : p.scale0) + (tile * p.groups + g0) * group_bytes, ng * group_bytes,
-                      &c.full[stage]);
-          }
-          issued_mask |= 1u << stage;
-          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
-        }
-      }
-      if (!ok) {
-        // let every copy in flight land before the CTA exits
-        for (int i = 0; i < p.stages; ++i) {
-          if (!(issued_mask & (1u << i))) continue;
-          const uint32_t par = (issued_parity >> i) & 1u;
-          const uint64_t t0 = globaltimer_ns();
-          while (!mbar_try_wait(&c.full[i], par) && globaltimer_ns() - t0 < 100000000ull) {
-          }
-        }
+      uint64_t* bar = &c.full[warp][pstage];
+      uint8_t* stage = ring + pstage * p.stage_bytes;
+      const int g0 = (pb * 64) >> p.group_shift;
+      const int ng = min(((pb + nb) * 64 - 1) >> p.group_shift, p.groups - 1) - g0 + 1;
+      const uint32_t data_bytes = nb * kBlockBytes, scale_bytes = static_cast<uint32_t>(ng * 16) << p.scale_shift;
+      mbar_arrive_expect_tx(bar, (data_bytes + scale_bytes) * ptiles * (kSwiglu ? 2 : 1));
+#pragma unroll
+      for (int m = 0; m < kMt; ++m) {
+        const bool up = kSwiglu && m >= kOutMt;
+        const int t = up ? m - kOutMt : m;
+        if (kOutMt > 1 && t >= ptiles) continue;
+        bulk_load(stage + m * p.chunk * kBlockBytes,
+                  (up ? p.data1 : p.data0) + (static_cast<int64_t>(ptile + t) * p.kb + pb) * kBlockBytes, data_bytes,
+                  bar);
+        bulk_load(stage + kMt * p.chunk * kBlockBytes + m * p.scale_slot,
+                  (up ? p.scale1 : p.scale0) +
+                      ((static_cast<int64_t>(ptile + t) * p.groups + g0) << (4 + p.scale_shift)),
+                  scale_bytes, bar);
       }
     }
-    return;
-  }
-  // -------------------------------------------------------------- MMA warps
+    if (++pstage == static_cast<uint32_t>(p.stages)) pstage = 0;
+    pb += nb;
+    if (pb == hi) {
+      pb = lo;
+      pu += kStep;
+      if (pu < u1) place();
+    }
+  };
+  for (int i = 0; i < p.stages && pu < u1; ++i) issue();
+
+  // ---------------------------------------------------------------- products
   const int g = lane >> 2, q = lane & 3;
+  const int full_blocks = p.K / 64;  // blocks without columns past K
   uint32_t stage = 0, phase = 0;
-  int buf = 0;
+  int buf = 0, at = at0;
   bool ok = true;
-  for (int u = u0; u < u1; ++u) {
-    const Unit r = locate(u);
-    const int tiles = min(kOutTiles, p.n16 - r.tile0);
-    float acc[kMt][kNt][4];
+  for (int u = u0; u < u1; u += kStep) {
+    const Unit r = locate(u, at);
+    // this lane's pieces of its tokens' rows (token 8 j + g; past the unit's
+    // rows another of its rows, whose sums are not stored)
+    const uint4* xp[kNt];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+      xp[j] = reinterpret_cast<const uint4*>(
+          p.x + static_cast<int64_t>(r.row0 + min(8 * j + g, r.rows - 1)) * p.K + 64 * lo + 8 * q);
+    // Two sets of x values, loaded a block ahead, where the registers allow; else one.
+    constexpr int kSets = kNt == 1 ? 2 : 1;
+    uint4 xv[kSets][kNt][2];
+    auto load_x = [&](uint4 (&v)[2], int j) {  // whole blocks; and on to the next
+      v[0] = xp[j][0];
+      v[1] = xp[j][4];
+      xp[j] += 8;
+    };
+    float part[kMt][kNt][4];
 #pragma unroll
     for (int m = 0; m < kMt; ++m)
 #pragma unroll
       for (int j = 0; j < kNt; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.f;
-    for (int s = 0; ok && s < stages_per_unit; ++s) {
-      const int b = s * kWarps + warp;
-      // this lane's pieces of its tokens' rows (token 8 j + g): before the wait
-      uint4 xv[kNt][2];
+        for (int e = 0; e < 4; ++e) part[m][j][e] = 0.f;
+    // The sums of the ranges so far (kSplit false): in registers where they are few, else in shared memory.
+    constexpr bool kTotRegs = kMt * kNt <= 2;
+    float tot[kTotRegs ? kMt : 1][kTotRegs ? kNt : 1][4];
+    float* mine = sums + buf * (S::kBytes / 4) + warp * kMt * kNt * 4 * 32 + lane;
+    int boundary = range;  // the end of the range being summed
+#pragma unroll
+    for (int m = 0; m < kMt; ++m)
 #pragma unroll
       for (int j = 0; j < kNt; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          xv[j][h] = make_uint4(0, 0, 0, 0);
-          const int col = 64 * b + 32 * h + 8 * q;
-          if (8 * j + g < r.rows && col < p.K)
-            xv[j][h] = *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(r.row0 + 8 * j + g) * p.K + col);
+        for (int e = 0; e < 4; ++e) {
+          if (kTotRegs) tot[kTotRegs ? m : 0][kTotRegs ? j : 0][e] = 0.f;
+          else mine[((m * kNt + j) * 4 + e) * 32] = 0.f;
         }
-      const bool got = wait_parity_bounded(&c.full[stage], phase, abort_flag, p.status);
-      if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
-      if (b < p.kb) {
-        const uint8_t* data = ring + stage * stage_bytes + warp * kBlockBytes + lane * 16;
-        const uint8_t* scales = ring + stage * stage_bytes + Sh::kDataStage;
+    const uint4* codes_at = nullptr;   // of the stage: this lane's codes of its first block ...
+    const float* scales_at = nullptr;  // ... and the f32 scales of its first row
+    int b0 = lo, g0 = 0;
+    // block b of the stage, with the x values v; loads the set `to` of block b + 1 of kSets 1
+    auto product = [&](int b, uint4 (&v)[kNt][2], bool more) {
+      constexpr int kParts = kG32 ? 2 : 1;  // scaled sums per block
 #pragma unroll
-        for (int m = 0; m < kMt; ++m) {
-          if (kSwiglu ? (m % kOutTiles) >= tiles : m >= tiles) continue;
-          const uint4 codes = *reinterpret_cast<const uint4*>(data + m * kTileStage);
-          const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
-          constexpr int kParts = kG32 ? 2 : 1;  // scaled sums per block
-          float sc[kParts][2];
+      for (int m = 0; m < kMt; ++m) {
+        // tiles past N were not copied: their sums are not stored
+        const uint4 codes = codes_at[(m * p.chunk + b - b0) * (kBlockBytes / 16)];
+        const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+        float sc[kParts][2];
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+          // (of a half block past the last group, what lies there: its sum is 0 and is left out)
+          const float* at_group = scales_at + m * (p.f32_slot / 4) + (((64 * b + 32 * h) >> p.group_shift) - g0) * 16;
+          sc[h][0] = at_group[0];
+          sc[h][1] = at_group[8];
+        }
+        uint32_t a[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes_to_a<kF16>(word[i], a[i]);
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+          if (kNt > 1 && 8 * j >= r.rows) continue;
 #pragma unroll
           for (int h = 0; h < kParts; ++h) {
-            const int gi = ((64 * warp + 32 * h) >> p.group_shift) * 16 + g;
-            const uint8_t* at_tile = scales + m * (scale_stage / kMt);
-            // the second half of K's last block may lie past the last group: nothing was copied for it
-            const bool has = !kG32 || (64 * b + 32 * h) < p.K;
-            sc[h][0] = has ? norm::load_one(at_tile, p.scale_dt, gi) : 0.f;
-            sc[h][1] = has ? norm::load_one(at_tile, p.scale_dt, gi + 8) : 0.f;
-          }
-          uint32_t a[4][4];
+            float d[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) codes_to_a<kF16>(word[i], a[i]);
-#pragma unroll
-          for (int j = 0; j < kNt; ++j) {
-            if (8 * j >= r.rows) continue;
-#pragma unroll
-            for (int h = 0; h < kParts; ++h) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int i = 4 / kParts * h; i < 4 / kParts * (h + 1); ++i) {
-                const uint4& v = xv[j][i / 2];
-                if (i % 2 == 0) gemm::mma_16816(d, a[i], v.x, v.y, kF16);
-                else gemm::mma_16816(d, a[i], v.z, v.w, kF16);
-              }
-              acc[m][j][0] = fmaf(sc[h][0], d[0], acc[m][j][0]);
-              acc[m][j][1] = fmaf(sc[h][0], d[1], acc[m][j][1]);
-              acc[m][j][2] = fmaf(sc[h][1], d[2], acc[m][j][2]);
-              acc[m][j][3] = fmaf(sc[h][1], d[3], acc[m][j][3]);
+            for (int i = 4 / kParts * h; i < 4 / kParts * (h + 1); ++i) {
+              const uint4& w = v[j][i / 2];
+              const uint32_t x0 = i % 2 ? w.z : w.x, x1 = i % 2 ? w.w : w.y;
+              if (i % (4 / kParts) == 0) mma<kF16, true>(d, a[i], x0, x1);
+              else mma<kF16, false>(d, a[i], x0, x1);
             }
+            if (kG32 && 64 * b + 32 * h >= p.K) continue;
+            part[m][j][0] = fmaf(sc[h][0], d[0], part[m][j][0]);
+            part[m][j][1] = fmaf(sc[h][0], d[1], part[m][j][1]);
+            part[m][j][2] = fmaf(sc[h][1], d[2], part[m][j][2]);
+            part[m][j][3] = fmaf(sc[h][1], d[3], part[m][j][3]);
+          }
+          if (kSets == 1 && m == kMt - 1 && more) load_x(v[j], j);
+        }
+      }
+      if (!kSplit && b + 1 == boundary) {  // a range is done: add it to the sums so far
+#pragma unroll
+        for (int m = 0; m < kMt; ++m)
+#pragma unroll
+          for (int j = 0; j < kNt; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float& t = kTotRegs ? tot[kTotRegs ? m : 0][kTotRegs ? j : 0][e] : mine[((m * kNt + j) * 4 + e) * 32];
+              t += part[m][j][e];
+              part[m][j][e] = 0.f;
+            }
+        boundary += range;
+      }
+    };
+    const int whole = min(hi, full_blocks);  // the blocks before K's last columns, if those are this warp's
+    if (lo < whole) {
+#pragma unroll
+      for (int j = 0; j < kNt; ++j)
+        if (8 * j < r.rows) load_x(xv[0][j], j);
+    }
+    while (b0 < hi) {
+      const bool got = wait_parity_bounded(&c.full[warp][stage], phase, abort_flag, p.status);
+      if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+      const int b1 = min(hi, b0 + p.chunk);
+      const uint8_t* here = ring + stage * p.stage_bytes;
+      codes_at = reinterpret_cast<const uint4*>(here) + lane;
+      scales_at = reinterpret_cast<const float*>(here + kMt * p.chunk * kBlockBytes) + g;
+      g0 = (b0 * 64) >> p.group_shift;
+      if (p.scale_dt != MOE_DT_F32) {  // once per stage: the scales as f32, into the warp's own copy
+        const int n = (min((b1 * 64 - 1) >> p.group_shift, p.groups - 1) - g0 + 1) * 16;
+#pragma unroll
+        for (int m = 0; m < kMt; ++m)
+          for (int i = lane; i < n; i += 32)
+            f32_scales[m * (p.f32_slot / 4) + i] =
+                norm::load_one(here + kMt * p.chunk * kBlockBytes + m * p.scale_slot, p.scale_dt, i);
+        scales_at = f32_scales + g;
+        __syncwarp();
+      }
+      int b = b0;
+      const int stop = min(b1, whole);
+      if (kSets == 2) {
+        // pairs of blocks, each set of x loaded while the other is used; a stage of odd length ends on a copy
+#pragma unroll 1
+        for (; b + 1 < stop; b += 2) {
+          load_x(xv[1][0], 0);
+          product(b, xv[0], false);
+          if (b + 2 < whole) load_x(xv[0][0], 0);
+          product(b + 1, xv[1 % kSets], false);
+        }
+        if (b < stop) {
+          if (b + 1 < whole) load_x(xv[1 % kSets][0], 0);
+          product(b, xv[0], false);
+          xv[0][0][0] = xv[1 % kSets][0][0];
+          xv[0][0][1] = xv[1 % kSets][0][1];
+          ++b;
+        }
+      } else {
+#pragma unroll 1
+        for (; b < stop; ++b) product(b, xv[0], b + 1 < whole);
+      }
+      if (b < b1) {  // K's last columns
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+          xv[0][j][0] = norm::load16_if(xp[j], 64 * b + 8 * q < p.K);
+          xv[0][j][1] = norm::load16_if(xp[j] + 4, 64 * b + 32 + 8 * q < p.K);
+        }
+        product(b, xv[0], false);
+      }
+      __syncwarp();  // the stage has been read: bring the one after the ring's others
+      if (pu < u1) issue();
+      if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
+      b0 = b1;
+    }
+    if (!kSplit) {
+      if (!ok) break;
+      // rows g, g + 8 of each tile, tokens 2 q, 2 q + 1 of each token tile
+#pragma unroll
+      for (int m = 0; m < kOutMt; ++m) {
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = 8 * j + 2 * q + (e & 1), ch = (r.tile0 + m) * 16 + g + ((e >> 1) << 3);
+            if (tok >= r.rows || ch >= p.N) continue;
+            auto total = [&](int t) {
+              const float before = kTotRegs ? tot[kTotRegs ? t : 0][kTotRegs ? j : 0][e] : mine[((t * kNt + j) * 4 + e) * 32];
+              return before + part[t][j][e];
+            };
+            float v = total(m);
+            if (kSwiglu) v = v / (1.0f + __expf(-v)) * total(kMt - kOutMt + m);
+            p.out[(r.row0 + tok) * p.ldo + ch] = static_cast<uint16_t>(gemm::pack2(v, 0.f, kF16) & 0xFFFFu);
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c.empty[stage]);
+    } else {
+#pragma unroll
+      for (int m = 0; m < kMt; ++m)
+#pragma unroll
+        for (int j = 0; j < kNt; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine[((m * kNt + j) * 4 + e) * 32] = part[m][j][e];
+      // all warps go on together or not at all
+      ok = named_bar_and(1, kThreads, ok);
+      if (!ok) break;
+      const float* slab = sums + buf * (S::kBytes / 4);
+      auto total = [&](int m, int n, int tok) {  // row n (0 .. 15) of tile m, token tok
+        const int j = tok >> 3, e = ((n >> 3) << 1) | (tok & 1), l = ((n & 7) << 2) | ((tok & 7) >> 1);
+        const float* v = slab + ((m * kNt + j) * 4 + e) * 32 + l;
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          // an empty range adds nothing (its warp wrote zeros)
+          t += v[w * kMt * kNt * 4 * 32];
+        return t;
+      };
+      for (int i = tid; i < r.rows * kOutMt * 16; i += kThreads) {
+        const int tok = i / (kOutMt * 16), n = i % (kOutMt * 16);
+        const int ch = r.tile0 * 16 + n;
+        if (ch >= p.N) continue;
+        float v = total(n >> 4, n & 15, tok);
+        if (kSwiglu) v = v / (1.0f + __expf(-v)) * total(kOutMt + (n >> 4), n & 15, tok);
+        p.out[(r.row0 + tok) * p.ldo + ch] = static_cast<uint16_t>(gemm::pack2(v, 0.f, kF16) & 0xFFFFu);
+      }
+      buf ^= 1;
+    }
+  }
+  if (!ok && lane == 0) {
+    // let every copy in flight land before the CTA exits: the stages from here on
+    const uint64_t t0 = globaltimer_ns();
+    for (int i = 0; i < p.stages; ++i) {
+      while (!mbar_try_wait(&c.full[warp][stage], phase) && globaltimer_ns() - t0 < 100000000ull) {
+      }
       if (++stage == static_cast<uint32_t>(p.stages)) { stage = 0; phase ^= 1u; }
     }
-    // ---- join the warps' sums: element (tile m, token tile j, e) of lane l
-    float* slab = red + buf * (Sh::kRedBytes / 4);
-#pragma unroll
-    for (int m = 0; m < kMt; ++m)
-#pragma unroll
-      for (int j = 0; j < kNt; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) slab[(((warp * kMt + m) * kNt + j) * 4 + e) * 32 + lane] = acc[m][j][e];
-    // all warps leave together or not at all
-    ok = named_bar_and(1, 32 * kWarps, ok);
-    if (!ok) break;
-    auto total = [&](int m, int n, int tok) {  // row n (0 .. 15) of tile m, token tok
-      const int j = tok >> 3, e = ((n >> 3) << 1) | (tok & 1), l = ((n & 7) << 2) | ((tok & 7) >> 1);
-      float t = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) t += slab[(((w * kMt + m) * kNt + j) * 4 + e) * 32 + l];
-      return t;
-    };
-    for (int i = tid; i < r.rows * kOutTiles * 16; i += 32 * kWarps) {
-      const int tok = i / (kOutTiles * 16), n = i % (kOutTiles * 16);
-      const int ch = r.tile0 * 16 + n;
-      if (ch >= p.N) continue;
-      float v = total(n >> 4, n & 15, tok);
-      if (kSwiglu) {
-        const float up = total(kOutTiles + (n >> 4), n & 15, tok);
-        v = v / (1.0f + __expf(-v)) * up;
-      }
-      p.out[(r.row0 + tok) * p.ldo + ch] = static_cast<uint16_t>(gemm::pack2(v, 0.f, kF16) & 0xFFFFu);
-    }
-    buf ^= 1;
   }
 }
 
@@ -368,24 +511,44 @@ struct DequantParams {
   const uint8_t* scale;
   const int32_t* offsets;  // of the first expert: experts without rows are skipped
   uint16_t* out;         // (experts, N, K)
-  int N, K, n16, kb, groups, group_shift, scale_dt, scale_shift, f16;
+  int N, K, n16, kb, groups, group_shift, scale_dt;
 };
 
+// A pair of exact 16-bit values times s in f32, each rounded once.
+template <bool kF16>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t v, float s) {
+  float lo, hi;
+  if (kF16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    lo = f.x;
+    hi = f.y;
+  } else {
+    lo = __uint_as_float(v << 16);
+    hi = __uint_as_float(v & 0xFFFF0000u);
+  }
+  return gemm::pack2(lo * s, hi * s, kF16);
+}
+
 // One warp per 16 x 64 block: 16 bytes of codes per lane in, 4 x 16 bytes out
-// (two rows, two runs of 8 columns), each value code * scale rounded once.
+// (two rows, two runs of 8 columns), each value code * scale rounded once. The
+// codes become floats as in the products (integer conversions run at a
+// quarter of the rate).
+template <bool kF16>
 __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
   pdl_trigger();
   pdl_wait();  // before the first global memory access
-  const int e = blockIdx.y;
+  const int e = blockIdx.z;
   if (p.offsets[e + 1] <= p.offsets[e]) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t block = static_cast<int64_t>(blockIdx.x) * 8 + warp;
-  if (block >= static_cast<int64_t>(p.n16) * p.kb) return;
-  const int tile = static_cast<int>(block / p.kb), b = static_cast<int>(block % p.kb);
+  const int b = blockIdx.x * 8 + warp, tile = blockIdx.y;  // a CTA walks along K
+  if (b >= p.kb) return;
   const int64_t et = static_cast<int64_t>(e) * p.n16 + tile;
   const uint4 codes = *reinterpret_cast<const uint4*>(p.data + (et * p.kb + b) * kBlockBytes + lane * 16);
-  const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
   const int g = lane >> 2, q = lane & 3;
+  const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+  uint32_t a[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) codes_to_a<kF16>(word[i], a[i]);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int col = 64 * b + 32 * j + 8 * q;
@@ -396,16 +559,9 @@ __global__ void __launch_bounds__(256) dequant_kernel(const DequantParams p) {
       const int n = 16 * tile + 8 * h + g;
       if (n >= p.N) continue;
       const float s = norm::load_one(p.scale, p.scale_dt, gi + 8 * h);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // columns 2 i, 2 i + 1: step i / 2, pair i % 2
-        const uint32_t v = word[2 * j + i / 2] >> (8 * (i % 2) + 4 * h);
-        const float lo = static_cast<float>(static_cast<int>(v & 15u) - 8);
-        const float hi = static_cast<float>(static_cast<int>((v >> 16) & 15u) - 8);
-        w[i] = gemm::pack2(lo * s, hi * s, p.f16);
-      }
       *reinterpret_cast<uint4*>(p.out + (static_cast<int64_t>(e) * p.N + n) * p.K + col) =
-          make_uint4(w[0], w[1], w[2], w[3]);
+          make_uint4(scale_pair<kF16>(a[2 * j][h], s), scale_pair<kF16>(a[2 * j][2 + h], s),
+                     scale_pair<kF16>(a[2 * j + 1][h], s), scale_pair<kF16>(a[2 * j + 1][2 + h], s));
     }
   }
 }

@@ -22,6 +22,7 @@
 #include "gemm_warp.cuh"
 #include "group.cuh"
 #include "int4.cuh"
+#include "int4_tile.cuh"
 #include "norm.cuh"
 #include "permute.cuh"
 #include "route.cuh"
@@ -1943,8 +1944,10 @@ using Int4Kernel = void (*)(const moe::int4::Params);
 
 // Bytes of 16-bit weights made at a time for many rows per expert.
 constexpr int64_t kInt4ChunkBytes = 256ll << 20;
-// Shared memory of one direct CTA: two per SM, with room left for L1.
-constexpr size_t kInt4Smem = 96 * 1024;
+// Shared memory of an SM's direct CTAs, with room left for L1.
+constexpr int64_t kInt4Smem = 208 * 1024;
+// Blocks of 64 columns in a stage of a warp's ring, at most.
+constexpr int kInt4Chunk = 8;
 
 // One product: data1/scale1 are the up projection of a SwiGLU pair.
 struct Int4Spec {
@@ -1964,7 +1967,21 @@ int log2_of(int64_t v) {
   return s;
 }
 
-bool int4_direct(int64_t M, int64_t E) { return M <= MOE_INT4_DIRECT_ROWS * E; }
+// Which form multiplies M rows of E experts, by the rows of an average expert.
+// Measured on B200 (64 experts, 6 per token, 1408 x 2048; us; groups of 128 / 64 / 32):
+//   rows           1.5       6       8.7        12         24          48          64          96         128
+//   warp MMAs    37/37/37 44/42/46 59/57/80  60/58/81  90/85/116       -           -           -           -
+//   64-row tile  58/61/80 71/74/98 71/75/98 72/75/104 73/78/120  74/90/146  110/130/210 141/165/264 171/202/324
+//   128-row tile    -        -        -         -      91/134/236 98/153/264 104/163/281 107/182/326 169/297/553
+//   16 bits         -        -        -         -     154/157/161 155/158/162 156/159/163 158/161/165 180/183/186
+// (128 rows in 64-row tiles, 192 rows: 232 against 181 in 16 bits). Each scale group's sums pass
+// through TMEM, so shorter groups cost the tiles more; the 128-row tile pays for groups of 128 on.
+enum class Int4Form { kWarp, kTile64, kTile128, k16Bit };
+Int4Form int4_form(int64_t M, int64_t E, int group) {
+  if (M <= 12 * E) return Int4Form::kWarp;
+  if (M <= 48 * E) return Int4Form::kTile64;
+  return M <= MOE_INT4_EXACT_ROWS(group) * E ? Int4Form::kTile128 : Int4Form::k16Bit;
+}
 
 // Experts whose 16-bit weights (projections x N x K) are made at a time.
 int64_t int4_chunk(int64_t E, int64_t N, int64_t K, int projections) {
@@ -1973,8 +1990,8 @@ int64_t int4_chunk(int64_t E, int64_t N, int64_t K, int projections) {
   return n < 1 ? 1 : n > E ? E : n;
 }
 
-size_t int4_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int projections) {
-  if (M <= 0 || E <= 0 || N <= 0 || K <= 0 || int4_direct(M, E)) return 0;
+size_t int4_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int group, int projections) {
+  if (M <= 0 || E <= 0 || N <= 0 || K <= 0 || int4_form(M, E, group) != Int4Form::k16Bit) return 0;
   // each projection's weights start 256-byte aligned
   return static_cast<size_t>(projections) *
          ((static_cast<size_t>(int4_chunk(E, N, K, projections)) * N * K * 2 + 255) & ~size_t(255));
@@ -1996,47 +2013,56 @@ int check_int4(const Int4Spec& s) {
   return MOE_OK;
 }
 
-template <int kMt, int kNt, bool kSwiglu, bool kF16, bool kG32>
+template <int kMt, int kNt, bool kSplit, bool kSwiglu, bool kF16, bool kG32>
 int launch_int4(moe::int4::Params p, int64_t units, int sms, cudaStream_t stream) {
-  constexpr uint32_t fixed = moe::int4::fixed_smem<kMt, kNt>();
-  const uint32_t stage = moe::int4::Shape<kMt, kNt>::kDataStage +
-                         moe::int4::scale_stage_bytes(kMt, p.group_shift, p.scale_shift);
-  int64_t stages = (static_cast<int64_t>(kInt4Smem) - fixed) / stage;
+  constexpr int64_t fixed = moe::int4::Sums<kMt, kNt, kSplit>::kFixed;
+  constexpr int per_sm = moe::int4::ctas_per_sm(kNt);
+  constexpr int64_t smem = kInt4Smem / per_sm / 128 * 128;
+  // a warp's blocks of a unit, in stages of equal chunks: the longest of which two stages fit
+  const int run = kSplit ? (p.kb + moe::int4::kRanges - 1) / moe::int4::kRanges : p.kb;
+  int64_t stages = 0;
+  for (int per_unit = (run + kInt4Chunk - 1) / kInt4Chunk; stages < 2 && per_unit <= run; ++per_unit) {
+    p.chunk = (run + per_unit - 1) / per_unit;
+    // groups that a chunk touches: one more than its length where it may start inside a group
+    const int groups = (p.chunk * 64 + (1 << p.group_shift) - 1) / (1 << p.group_shift) + (p.group_shift > 6 ? 1 : 0);
+    p.scale_slot = groups * (16 << p.scale_shift);
+    p.stage_bytes = kMt * (p.chunk * moe::int4::kBlockBytes + p.scale_slot);
+    p.f32_slot = groups * 64;
+    stages = ((smem - fixed) / moe::int4::kWarps - kMt * p.f32_slot) / p.stage_bytes;
+  }
+  CHECK_ARG(stages >= 2, "int4 stages do not fit shared memory");
   stages = stages > moe::int4::kMaxStages ? moe::int4::kMaxStages : stages;
-  static_assert(fixed + 2 * (moe::int4::Shape<kMt, kNt>::kDataStage + kMt * 1024) <= kInt4Smem, "two stages fit");
   p.stages = static_cast<int>(stages);
-  const auto kernel = moe::int4::int4_kernel<kMt, kNt, kSwiglu, kF16, kG32>;
+  const auto kernel = moe::int4::int4_kernel<kMt, kNt, kSplit, kSwiglu, kF16, kG32>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kInt4Smem));
+    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   });
   if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(int4)");
-  const int64_t grid = units < 2 * sms ? units : 2 * sms;
-  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(moe::int4::kThreads), fixed + stages * stage,
-                      stream, p),
+  const int64_t want = kSplit ? units : (units + moe::int4::kWarps - 1) / moe::int4::kWarps;
+  const int64_t grid = want < per_sm * sms ? want : per_sm * sms;
+  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(moe::int4::kThreads),
+                      static_cast<size_t>(fixed + moe::int4::kWarps * (stages * p.stage_bytes + kMt * p.f32_slot)), stream, p),
            "int4_kernel launch");
   return MOE_OK;
 }
 
 template <bool kSwiglu, bool kF16, bool kG32>
 int launch_int4_shape(const moe::int4::Params& p, int64_t avg_rows, int sms, cudaStream_t stream) {
-  // at most this many (weight tile, token tile) pairs, in 16 x 8 tiles
-  const int64_t out_tiles = (kSwiglu ? 2 : 1) * static_cast<int64_t>(p.n16);
+  constexpr int kMt = kSwiglu ? 2 : 1;
+  // at most this many units, of mt weight tiles and 8 nt token rows
   auto units = [&](int mt, int nt) {
     const int64_t tok = p.M / (8 * nt) + (p.E < p.M ? p.E : p.M);
-    return tok * ((out_tiles + mt - 1) / mt);
+    return tok * (((kSwiglu ? 2 : 1) * static_cast<int64_t>(p.n16) + mt - 1) / mt);
   };
-  if (avg_rows > 8) return launch_int4<2, 4, kSwiglu, kF16, kG32>(p, units(2, 4), sms, stream);
-  if (avg_rows > 4) return launch_int4<2, 2, kSwiglu, kF16, kG32>(p, units(2, 2), sms, stream);
-  if constexpr (!kSwiglu) {
-    if (units(2, 1) < 4 * sms) return launch_int4<1, 1, kSwiglu, kF16, kG32>(p, units(1, 1), sms, stream);
-  }
-  return launch_int4<2, 1, kSwiglu, kF16, kG32>(p, units(2, 1), sms, stream);
+  if (avg_rows > 6) return launch_int4<2, 2, false, kSwiglu, kF16, kG32>(p, units(2, 2), sms, stream);
+  if (units(kMt, 1) < 8 * sms) return launch_int4<kMt, 1, true, kSwiglu, kF16, kG32>(p, units(kMt, 1), sms, stream);
+  return launch_int4<kMt, 1, false, kSwiglu, kF16, kG32>(p, units(kMt, 1), sms, stream);
 }
 
-template <bool kSwiglu>
-int run_int4_direct(const Int4Spec& s, int sms, int32_t* status, cudaStream_t stream) {
+// What both forms of the product share.
+moe::int4::Params int4_params(const Int4Spec& s, int32_t* status) {
   moe::int4::Params p{};
   p.data0 = static_cast<const uint8_t*>(s.data0);
   p.data1 = static_cast<const uint8_t*>(s.data1);
@@ -2057,13 +2083,62 @@ int run_int4_direct(const Int4Spec& s, int sms, int32_t* status, cudaStream_t st
   p.group_shift = log2_of(s.group);
   p.scale_dt = s.scale_dtype;
   p.scale_shift = s.scale_dtype == MOE_DT_F32 ? 2 : 1;
-  p.f16 = s.act_dtype == MOE_DT_F16;
+  return p;
+}
+
+template <bool kSwiglu>
+int run_int4_direct(const Int4Spec& s, int sms, int32_t* status, cudaStream_t stream) {
+  const moe::int4::Params p = int4_params(s, status);
   const int64_t avg = (s.M + s.E - 1) / s.E;
-  if (p.f16)
+  if (s.act_dtype == MOE_DT_F16)
     return s.group == 32 ? launch_int4_shape<kSwiglu, true, true>(p, avg, sms, stream)
                          : launch_int4_shape<kSwiglu, true, false>(p, avg, sms, stream);
   return s.group == 32 ? launch_int4_shape<kSwiglu, false, true>(p, avg, sms, stream)
                        : launch_int4_shape<kSwiglu, false, false>(p, avg, sms, stream);
+}
+
+template <bool kSwiglu, bool kF16, bool kG32, int kTok>
+int launch_int4_tile(const Int4Spec& s, int sms, int32_t* status, cudaStream_t stream) {
+  using Sh = moe::int4::TileShape<kTok>;
+  moe::int4::TileParams tp;
+  std::memset(&tp, 0, sizeof(tp));
+  tp.p = int4_params(s, status);
+  tp.nt = kTok;
+  int rc = make_map_a(&tp.map_x, s.x, s.act_dtype, s.M, s.K, s.K, kTok);
+  if (rc) return rc;
+  constexpr int64_t codes = static_cast<int64_t>(moe::int4::kConvWarps) * moe::int4::kCodeStages * Sh::kCodeChunk *
+                            moe::int4::kBlockBytes;
+  constexpr int64_t stage = Sh::kSub * (moe::int4::kABytes + kTok * 128);
+  constexpr int64_t fit = (static_cast<int64_t>(kMaxDynSmem) - moe::int4::tile_fixed_smem() - codes) / stage;
+  static_assert(fit >= Sh::kBatch, "a converter's batch fits the ring");
+  tp.tile_stages = static_cast<int>(fit > moe::int4::kTileStages ? moe::int4::kTileStages : fit);
+  const size_t smem = moe::int4::tile_fixed_smem() + tp.tile_stages * stage + codes;
+  const auto kernel = moe::int4::int4_tile_kernel<kSwiglu, kF16, kG32, kTok>;
+  static std::once_flag once;
+  static cudaError_t attr_err = cudaSuccess;
+  std::call_once(once, [&] {
+    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem));
+  });
+  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(int4 tile)");
+  const int64_t tok = s.M / kTok + (s.E < s.M ? s.E : s.M);
+  const int out_tiles = kSwiglu ? 4 : 8;
+  const int64_t tiles = tok * ((tp.p.n16 + out_tiles - 1) / out_tiles);
+  CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), dim3(Sh::kThreads), smem, stream,
+                      tp),
+           "int4_tile_kernel launch");
+  return MOE_OK;
+}
+
+template <bool kSwiglu, int kTok>
+int run_int4_tile(const Int4Spec& s, int sms, int32_t* status, cudaStream_t stream) {
+  const bool f16 = s.act_dtype == MOE_DT_F16;
+  if constexpr (kTok == 64) {
+    if (s.group == 32)
+      return f16 ? launch_int4_tile<kSwiglu, true, true, kTok>(s, sms, status, stream)
+                 : launch_int4_tile<kSwiglu, false, true, kTok>(s, sms, status, stream);
+  }
+  return f16 ? launch_int4_tile<kSwiglu, true, false, kTok>(s, sms, status, stream)
+             : launch_int4_tile<kSwiglu, false, false, kTok>(s, sms, status, stream);
 }
 
 int run_dequant(const Int4Spec& s, const void* data, const void* scale, int64_t e0, int64_t experts, void* out,
@@ -2076,15 +2151,14 @@ int run_dequant(const Int4Spec& s, const void* data, const void* scale, int64_t 
   p.groups = static_cast<int>((s.K + s.group - 1) / s.group);
   p.group_shift = log2_of(s.group);
   p.scale_dt = s.scale_dtype;
-  p.scale_shift = s.scale_dtype == MOE_DT_F32 ? 2 : 1;
-  p.f16 = s.act_dtype == MOE_DT_F16;
+  const int scale_shift = s.scale_dtype == MOE_DT_F32 ? 2 : 1;
   p.data = static_cast<const uint8_t*>(data) + e0 * p.n16 * p.kb * moe::int4::kBlockBytes;
-  p.scale = static_cast<const uint8_t*>(scale) + ((e0 * p.n16 * p.groups * 16) << p.scale_shift);
+  p.scale = static_cast<const uint8_t*>(scale) + ((e0 * p.n16 * p.groups * 16) << scale_shift);
   p.offsets = s.offsets + e0;
   p.out = static_cast<uint16_t*>(out);
-  const int64_t blocks = (static_cast<int64_t>(p.n16) * p.kb + 7) / 8;
-  CUDA_TRY(launch_pdl(moe::int4::dequant_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(experts)),
-                      dim3(256), 0, stream, p),
+  const dim3 grid(static_cast<unsigned>((p.kb + 7) / 8), static_cast<unsigned>(p.n16), static_cast<unsigned>(experts));
+  CUDA_TRY(launch_pdl(s.act_dtype == MOE_DT_F16 ? moe::int4::dequant_kernel<true> : moe::int4::dequant_kernel<false>,
+                      grid, dim3(256), 0, stream, p),
            "dequant_kernel launch");
   return MOE_OK;
 }
@@ -2096,10 +2170,15 @@ int run_int4(const Int4Spec& s, void* workspace, size_t workspace_bytes, int32_t
   rc = check_int4(s);
   if (rc || s.M == 0) return rc;
   const bool swiglu = s.data1 != nullptr;
-  if (int4_direct(s.M, s.E))
+  const Int4Form form = int4_form(s.M, s.E, s.group);
+  if (form == Int4Form::kWarp)
     return swiglu ? run_int4_direct<true>(s, sms, status, stream) : run_int4_direct<false>(s, sms, status, stream);
+  if (form == Int4Form::kTile64)
+    return swiglu ? run_int4_tile<true, 64>(s, sms, status, stream) : run_int4_tile<false, 64>(s, sms, status, stream);
+  if (form == Int4Form::kTile128)
+    return swiglu ? run_int4_tile<true, 128>(s, sms, status, stream) : run_int4_tile<false, 128>(s, sms, status, stream);
   const int projections = swiglu ? 2 : 1;
-  const size_t need = int4_bytes(s.M, s.E, s.N, s.K, projections);
+  const size_t need = int4_bytes(s.M, s.E, s.N, s.K, s.group, projections);
   CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace too small (%zu < %zu)",
             workspace_bytes, need);
   const int64_t chunk = int4_chunk(s.E, s.N, s.K, projections);
@@ -2135,7 +2214,9 @@ int run_int4(const Int4Spec& s, void* workspace, size_t workspace_bytes, int32_t
 
 extern "C" {
 
-size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K) { return int4_bytes(M, E, N, K, 1); }
+size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int group) {
+  return int4_bytes(M, E, N, K, group, 1);
+}
 
 int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, const void* data, const void* scale,
                           int scale_dtype, int group, int64_t E, int64_t N, const int32_t* offsets, void* out,
@@ -2157,9 +2238,9 @@ int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, cons
   return run_int4(s, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
-size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I) {
+size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I, int group) {
   if (R <= 0 || I <= 0) return 0;
-  const size_t a = int4_bytes(R, E, I, H, 2), b = int4_bytes(R, E, H, I, 1);
+  const size_t a = int4_bytes(R, E, I, H, group, 2), b = int4_bytes(R, E, H, I, group, 1);
   return ((static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255)) + (a > b ? a : b);
 }
 
@@ -2170,7 +2251,7 @@ int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, con
   if (R == 0) return MOE_OK;
   CHECK_ARG(gate && up && down, "null pointer");
   CHECK_ARG(I >= 8 && I % 8 == 0, "I=%lld must be a multiple of 8", (long long)I);
-  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= moe_ffn_int4_workspace_bytes(R, E, H, I),
+  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= moe_ffn_int4_workspace_bytes(R, E, H, I, group),
             "workspace too small");
   const size_t h_bytes = (static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255);
   char* rest = static_cast<char*>(workspace) + h_bytes;

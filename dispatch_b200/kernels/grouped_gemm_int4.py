@@ -2,11 +2,12 @@
 int8 contract of ``grouped_gemm_int8.py`` for ``Int4Tensor`` weights. No
 reference counterpart.
 
-Groups averaging up to 32 rows (decode) multiply the codes directly: laid out
-weights stream through shared memory once, the codes become 16-bit floats
-exactly in the MMA's registers and each column group's f32 sum is multiplied by
-its scale. Larger batches write the weights as 16-bit tiles, a few experts at a
-time, for the tcgen05 kernels (one rounding of code * scale per weight)."""
+Up to 128 rows per expert on average (48 with groups below 128) the codes
+themselves are multiplied: they become 16-bit floats exactly on the way to the
+tensor cores (warp-level MMAs for a few rows, tcgen05 for more) and each column
+group's f32 sum is multiplied by its scale. Larger batches write the weights as
+16-bit ones, some experts at a time, for the 16-bit tcgen05 kernels (one
+rounding of code * scale per weight)."""
 
 from __future__ import annotations
 
@@ -59,7 +60,7 @@ def grouped_matmul_int4(x: torch.Tensor, qweight: Int4Tensor, schedule: TileSche
     x = _aligned(x)
     offsets = device_offsets(schedule, dev)
     lib = L.lib()
-    ws = _workspace(lib.moe_int4_workspace_bytes(m, e, qweight.n, qweight.k), dev)
+    ws = _workspace(lib.moe_int4_workspace_bytes(m, e, qweight.n, qweight.k, qweight.group_size), dev)
     L.call(
         "grouped_matmul_int4", dev, lib.moe_grouped_gemm_int4,
         x.data_ptr(), L.dt(x), m, qweight.k, qweight.data.data_ptr(), qweight.scale.data_ptr(),
@@ -89,7 +90,7 @@ def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4Stacke
     r, h, i, e = xs.shape[0], gate.k, gate.n, gate.num_experts
     y = torch.empty(r, h, dtype=xs.dtype, device=dev)
     lib = L.lib()
-    ws = _workspace(lib.moe_ffn_int4_workspace_bytes(r, e, h, i), dev)
+    ws = _workspace(lib.moe_ffn_int4_workspace_bytes(r, e, h, i, gate.group_size), dev)
     L.call(
         "expert_ffn_int4", dev, lib.moe_expert_ffn_int4,
         xs.data_ptr(), L.dt(xs), r, h, offsets.contiguous().data_ptr(), e, i, gate.data.data_ptr(),

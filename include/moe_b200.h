@@ -391,16 +391,16 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
  * absmax / 7 in f32 (1 for a group of zeros) rounded to scale_dtype, code =
  * clamp(round_half_even(w / scale), -8, 7).
  *
- * Groups averaging at most MOE_INT4_DIRECT_ROWS rows multiply the codes
- * themselves (no weight is rounded, no workspace). Beyond that the weights of
- * as many experts as fit the workspace at a time are written as code * scale
- * rounded to x's type and multiplied on the tcgen05 kernels; f16 then holds
- * them in f16's range, as it does f16 weights. workspace:
- * moe_int4_workspace_bytes (0 for a direct call), 16-byte aligned, no
- * initialisation. x (M, K) and out (M, ldo) bf16 or f16.
+ * Experts averaging at most MOE_INT4_EXACT_ROWS(group) rows multiply the
+ * codes themselves: no weight is rounded, no workspace.
+ * Beyond that the weights of as many experts as fit the workspace at a time
+ * are written as code * scale rounded to x's type and multiplied on the 16-bit
+ * tcgen05 kernels; f16 then holds them in f16's range, as it does f16 weights.
+ * workspace: moe_int4_workspace_bytes (0 where none is needed), 16-byte
+ * aligned, no initialisation. x (M, K) and out (M, ldo) bf16 or f16.
  */
-#define MOE_INT4_DIRECT_ROWS 32
-size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K);
+#define MOE_INT4_EXACT_ROWS(group) ((group) >= 128 ? 128 : 48)
+size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int group);
 int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, const void* data, const void* scale,
                           int scale_dtype, int group, int64_t E, int64_t N, const int32_t* offsets, void* out,
                           int64_t ldo, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
@@ -410,7 +410,7 @@ int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, cons
  * (E, H, I) laid out, one group size and scale type for the three. The
  * intermediate rows are in xs' type (in the workspace), SwiGLU in f32.
  */
-size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I);
+size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I, int group);
 int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, const int32_t* offsets, int64_t E,
                         int64_t I, const void* gate, const void* gate_scale, const void* up, const void* up_scale,
                         const void* down, const void* down_scale, int scale_dtype, int group, void* y,

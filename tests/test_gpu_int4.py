@@ -3,9 +3,10 @@
 Tolerances: an output is rounded once to its type (half a step of the value);
 f32 accumulation in MMA steps of 16 columns, each off by at most one unit 2u =
 2^-23 of the magnitudes added up so far, and a few products and joins: K / 8 +
-64 times u = 2^-24 of sum |x w|. With many rows per expert a weight is first
-rounded to x's type: the reference does the same. The FFN's intermediate rows
-are rounded to x's type: half a step of each, through the down weights."""
+64 times u = 2^-24 of sum |x w|. With many rows per expert each weight is rounded
+once to x's type, which the formula's weights follow; else none is. The FFN's
+intermediate rows are rounded to x's type: half a step of each, through the down
+weights."""
 
 from __future__ import annotations
 
@@ -42,7 +43,6 @@ from dispatch_b200.kernels.tile_schedule import build_tile_schedule  # noqa: E40
 DEV = torch.device("cuda", 0)
 U = 2.0**-24
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
-DIRECT_ROWS = 32  # MOE_INT4_DIRECT_ROWS
 
 
 @pytest.fixture(autouse=True)
@@ -62,11 +62,16 @@ def make(e, n, k, group, scale_dtype=F32, seed=0):
     return pack_int4(codes, scale, group), g
 
 
-def weights64(q, rows, dtype):
-    """The weights that a call with this many rows multiplies, in 64 bits."""
+def exact_rows(group):
+    """MOE_INT4_EXACT_ROWS: the codes themselves are multiplied up to this average."""
+    return 128 if group >= 128 else 48
+
+
+def weights64(q, rows=0, dtype=None):
+    """The formula's weights for a product of `rows` rows."""
     codes, scale = unpack_int4(q)
     w = codes.double() * scale.double().repeat_interleave(q.group_size, 2)[..., :q.k]
-    return w if rows <= DIRECT_ROWS * q.num_experts else w.float().to(dtype).double()
+    return w if rows <= exact_rows(q.group_size) * q.num_experts else w.to(dtype).double()
 
 
 def check(actual, value, bound):
@@ -77,8 +82,7 @@ def check(actual, value, bound):
 
 
 def check_product(out, x, q, offsets):
-    rows = x.shape[0]
-    w = weights64(q, rows, x.dtype)
+    w = weights64(q, x.shape[0], x.dtype)
     for e in range(q.num_experts):
         a, b = offsets[e], offsets[e + 1]
         if b > a:
@@ -101,41 +105,64 @@ def run(sizes, n, k, group, dtype=BF16, scale_dtype=F32, seed=0):
 @pytest.mark.parametrize("group", [32, 64, 128, 256])
 @pytest.mark.parametrize(("sizes", "n", "k"), [
     ([1], 16, 64), ([1], 1, 8), ([0, 1, 0], 17, 72), ([3, 0, 1, 8, 9], 100, 1416), ([1] * 6, 1408, 2048),
-    ([5, 6, 0, 7], 250, 520), ([16, 33, 0, 2], 72, 264), ([70, 1], 48, 136), ([2, 0], 33, 4168),
+    ([5, 6, 0, 7], 250, 520), ([11, 33, 0, 2], 72, 264), ([23, 1], 48, 136), ([2, 0], 33, 4168),
 ])
-def test_direct_product(sizes, n, k, group, dtype) -> None:
-    assert sum(sizes) <= DIRECT_ROWS * len(sizes) or sizes == [70, 1]
+def test_few_rows(sizes, n, k, group, dtype) -> None:
+    assert sum(sizes) <= 12 * len(sizes)
+    run(sizes, n, k, group, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize(("sizes", "n", "k"), [
+    ([13], 16, 64), ([48], 1, 8), ([70, 1], 48, 136), ([0, 100, 0, 17], 17, 72), ([65, 0, 16, 30, 129], 100, 1416),
+    ([40] * 3, 1408, 2048), ([300, 0, 1, 0, 2, 0, 5], 250, 520),
+])
+def test_tiles_of_64_rows(sizes, n, k, group, dtype) -> None:
+    assert 12 * len(sizes) < sum(sizes) <= 48 * len(sizes)
+    run(sizes, n, k, group, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("group", [128, 256])
+@pytest.mark.parametrize(("sizes", "n", "k"), [
+    ([65], 16, 64), ([49], 48, 136), ([128], 1, 8), ([0, 250], 17, 72), ([130, 0, 256, 33, 129], 100, 1416), ([100] * 3, 1408, 2048),
+    ([300, 0, 1, 200], 250, 520),
+])
+def test_tiles_of_128_rows(sizes, n, k, group, dtype) -> None:
+    assert 48 * len(sizes) < sum(sizes) <= exact_rows(group) * len(sizes)
     run(sizes, n, k, group, dtype)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize(("sizes", "n", "k", "group"), [
-    ([33], 16, 64, 32), ([300, 0, 1, 257], 136, 520, 64), ([512, 512], 256, 264, 128), ([70, 0, 200], 17, 72, 256),
-    ([400, 330, 900], 2048, 1408, 128),
+    ([65], 16, 64, 32), ([300, 0, 1, 257], 136, 520, 64), ([512, 512], 256, 264, 128), ([170, 0, 300], 17, 72, 256),
+    ([400, 330, 900], 2048, 1408, 128), ([90, 40, 100], 72, 456, 32),
 ])
-def test_product_with_many_rows(sizes, n, k, group, dtype) -> None:
-    assert sum(sizes) > DIRECT_ROWS * len(sizes)
+def test_many_rows(sizes, n, k, group, dtype) -> None:
+    assert sum(sizes) > exact_rows(group) * len(sizes)
     run(sizes, n, k, group, dtype)
 
 
 @pytest.mark.parametrize("scale_dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("sizes", [[2, 5, 1], [90, 40, 3]])
+@pytest.mark.parametrize("sizes", [[2, 5, 1], [90, 40, 3], [190, 40, 13], [300, 100]])
 def test_scale_types(sizes, scale_dtype) -> None:
     for group in (32, 128):
         run(sizes, 80, 456, group, BF16, scale_dtype)
         run(sizes, 80, 456, group, F16, scale_dtype)
 
 
-@pytest.mark.parametrize("rows", [31, 32, 33, 34])
-def test_around_the_change_of_kernels(rows) -> None:
-    run([rows] * 3, 96, 256, 64)
+@pytest.mark.parametrize("group", [64, 128])
+@pytest.mark.parametrize("rows", [6, 7, 12, 13, 48, 49, 128, 129])
+def test_around_the_change_of_kernels(rows, group) -> None:
+    run([rows] * 3, 96, 256, group)
 
 
 def test_experts_made_in_several_chunks() -> None:
     """16-bit weights of 4 experts at most fit the workspace at a time."""
-    sizes = [40, 0, 33, 70, 90, 1, 33, 60, 35]
+    sizes = [140, 0, 133, 270, 190, 1, 133, 160, 136]
     n, k = 8192, 4096
-    ws = L.lib().moe_int4_workspace_bytes(sum(sizes), len(sizes), n, k)
+    ws = L.lib().moe_int4_workspace_bytes(sum(sizes), len(sizes), n, k, 128)
     assert 0 < ws < len(sizes) * n * k * 2
     run(sizes, n, k, 128)
 
@@ -143,7 +170,7 @@ def test_experts_made_in_several_chunks() -> None:
 def test_a_row_does_not_depend_on_its_batch() -> None:
     x, q, _, out = run([1, 4, 2], 144, 1096, 64, seed=4)
     one = x[4:5]  # of expert 1
-    for sizes, at in (([0, 1, 0], 0), ([3, 9, 0], 7), ([8, 20, 8], 20), ([30, 32, 30], 47)):
+    for sizes, at in (([0, 1, 0], 0), ([3, 9, 0], 7), ([8, 20, 8], 20), ([2, 32, 2], 30)):
         g = torch.Generator(device="cuda").manual_seed(sum(sizes))
         batch = torch.randn(sum(sizes), 1096, generator=g, device=DEV).to(BF16)
         batch[at] = one
@@ -157,16 +184,38 @@ def test_every_code_and_non_finite_rows() -> None:
     codes[0, 1:] = codes[0, 1:].flip(1)
     scale = torch.ones(1, 16, 1)
     scale[0, 3] = 0.0
-    q = pack_int4(codes.to(DEV), scale.to(DEV), 64)
+    q = pack_int4(codes.to(DEV), scale.to(DEV), 128)
     for dtype in (BF16, F16):
         x = torch.eye(k, device=DEV).to(dtype)  # column k of the weights, exactly
-        for rows in (32, 64):
-            out = grouped_matmul_int4(x[:rows], q, build_tile_schedule(torch.tensor([rows]), 16))
-            assert torch.equal(out, (codes[0].float() * scale[0]).t()[:rows].to(DEV, dtype))
-        x = torch.ones(5, k, device=DEV, dtype=dtype)
-        x[1, 3], x[3, 60] = float("inf"), float("nan")
-        out = grouped_matmul_int4(x, q, build_tile_schedule(torch.tensor([5]), 16))
-        assert torch.isfinite(out[[0, 2, 4]]).all() and torch.isnan(out[3]).all() and not torch.isfinite(out[1]).all()
+        for rows in (12, 48, 128, 192):
+            x_rows = x.repeat(3, 1)[:rows]
+            out = grouped_matmul_int4(x_rows, q, build_tile_schedule(torch.tensor([rows]), 16))
+            assert torch.equal(out, (codes[0].float() * scale[0]).t().repeat(3, 1)[:rows].to(DEV, dtype))
+        for rows in (5, 20, 100, 150):  # a row's infinities and NaN are its own
+            x_rows = torch.ones(rows, k, device=DEV, dtype=dtype)
+            x_rows[1, 3], x_rows[3, 60] = float("inf"), float("nan")
+            out = grouped_matmul_int4(x_rows, q, build_tile_schedule(torch.tensor([rows]), 16))
+            rest = [i for i in range(rows) if i not in (1, 3)]
+            assert torch.isfinite(out[rest]).all() and torch.isnan(out[3]).all() and not torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("rows", [5, 20, 100, 150])
+def test_rows_past_the_last_expert_are_left_alone(rows) -> None:
+    q, g = make(1, 40, 128, 128)
+    x = torch.randn(rows + 9, 128, generator=g, device=DEV).to(BF16)
+    x[rows:] = float("nan")
+    out = torch.full((rows + 9, 40), 7.0, device=DEV, dtype=BF16)
+    off = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    ws = torch.empty(max(L.lib().moe_int4_workspace_bytes(rows + 9, 1, 40, 128, 128), 16), dtype=torch.uint8, device=DEV)
+    rc = L.lib().moe_grouped_gemm_int4(
+        x.data_ptr(), L.DT_BF16, rows + 9, 128, q.data.data_ptr(), q.scale.data_ptr(), L.DT_F32, 128, 1, 40,
+        off.data_ptr(), out.data_ptr(), 40, ws.data_ptr(), ws.numel(), L.status_word(DEV).data_ptr(),
+        L.stream_ptr(DEV))
+    assert rc == L.MOE_OK
+    w = weights64(q, rows + 9, BF16)[0]
+    xe = x[:rows].double()
+    check(out[:rows], xe @ w.t(), deep(128) * (xe.abs() @ w.t().abs()))
+    assert bool((out[rows:] == 7.0).all())
 
 
 def test_strided_and_unaligned_rows() -> None:
@@ -189,7 +238,7 @@ def test_weights_past_4_gib() -> None:
     data = torch.randint(-2**31, 2**31 - 1, (e, n // 16, k // 64, 32, 4), dtype=torch.int32, device=DEV)
     assert data.numel() * 4 > 2**32
     scale = torch.full((e, n // 16, k // group, 16), 1 / 64, device=DEV, dtype=BF16)
-    for last in (3, 200):  # direct, and with few busy experts of a large batch
+    for last in (3, 4000):  # a few rows, and a batch of tiles
         sizes = [0] * e
         sizes[0], sizes[255] = 2, last
         x = torch.randn(sum(sizes), k, device=DEV).to(BF16)
@@ -197,20 +246,20 @@ def test_weights_past_4_gib() -> None:
         out = grouped_matmul_int4(x, Int4Tensor(data, scale, n, k, group), sched)
         for i, a, b in ((0, 0, 2), (255, 2, 2 + last)):
             one = Int4Tensor(data[i:i + 1], scale[i:i + 1], n, k, group)
-            w = weights64(one, 1, BF16)[0]
+            w = weights64(one)[0]
             check(out[a:b], x[a:b].double() @ w.t(), deep(k) * (x[a:b].double().abs() @ w.t().abs()))
 
 
 def test_bad_offsets_are_reported() -> None:
-    q, g = make(3, 40, 128, 64)
-    for rows in (6, 200):
+    q, g = make(3, 40, 128, 128)
+    for rows in (6, 100, 350, 500):
         x = torch.randn(rows, 128, generator=g, device=DEV).to(BF16)
         out = torch.full((rows, 40), 7.0, device=DEV, dtype=BF16)
-        ws = torch.empty(max(L.lib().moe_int4_workspace_bytes(rows, 3, 40, 128), 16), dtype=torch.uint8, device=DEV)
+        ws = torch.empty(max(L.lib().moe_int4_workspace_bytes(rows, 3, 40, 128, 128), 16), dtype=torch.uint8, device=DEV)
         for offsets in ([0, 2, 4, rows + 1], [0, 4, 2, rows], [-1, 2, 4, rows]):
             off = torch.tensor(offsets, dtype=torch.int32, device=DEV)
             rc = L.lib().moe_grouped_gemm_int4(
-                x.data_ptr(), L.DT_BF16, rows, 128, q.data.data_ptr(), q.scale.data_ptr(), L.DT_F32, 64, 3, 40,
+                x.data_ptr(), L.DT_BF16, rows, 128, q.data.data_ptr(), q.scale.data_ptr(), L.DT_F32, 128, 3, 40,
                 off.data_ptr(), out.data_ptr(), 40, ws.data_ptr(), ws.numel(), L.status_word(DEV).data_ptr(),
                 L.stream_ptr(DEV))
             assert rc == L.MOE_OK
@@ -272,7 +321,7 @@ def ffn_weights(e, i, h, group, scale_dtype=F32):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize(("sizes", "i", "h", "group"), [
     ([1, 0, 2], 24, 72, 32), ([6, 9, 0, 20], 136, 264, 64), ([1] * 6, 1408, 2048, 128), ([200, 0, 70], 104, 520, 128),
-    ([3, 1], 40, 128, 256),
+    ([3, 1], 40, 128, 256), ([40, 0, 100], 200, 264, 32), ([40, 0, 17, 100], 72, 520, 64), ([300, 133], 104, 264, 128),
 ])
 def test_expert_ffn(sizes, i, h, group, dtype) -> None:
     ws = ffn_weights(len(sizes), i, h, group)

@@ -102,11 +102,13 @@ def test_backends_and_workspaces() -> None:
     with pytest.raises(ValueError, match="bits"):
         resolve_quantized_backend(3)
     lib = L.lib()
-    assert lib.moe_int4_workspace_bytes(32 * 8, 8, 1408, 2048) == 0  # direct: no 16-bit weights
+    assert lib.moe_int4_workspace_bytes(128 * 8, 8, 1408, 2048, 128) == 0  # no 16-bit weights
+    assert lib.moe_int4_workspace_bytes(48 * 8, 8, 1408, 2048, 32) == 0
     per_expert = 1408 * 2048 * 2
-    assert lib.moe_int4_workspace_bytes(32 * 8 + 1, 8, 1408, 2048) >= per_expert
-    assert lib.moe_int4_workspace_bytes(10**6, 64, 2048, 1408) < 64 * per_expert  # made a few experts at a time
-    assert lib.moe_int4_workspace_bytes(0, 8, 1408, 2048) == 0
-    assert lib.moe_ffn_int4_workspace_bytes(6, 64, 2048, 1408) >= 6 * 1408 * 2
+    assert lib.moe_int4_workspace_bytes(128 * 8 + 1, 8, 1408, 2048, 128) >= per_expert
+    assert lib.moe_int4_workspace_bytes(48 * 8 + 1, 8, 1408, 2048, 64) >= per_expert
+    assert lib.moe_int4_workspace_bytes(10**6, 64, 2048, 1408, 64) < 64 * per_expert  # made a few experts at a time
+    assert lib.moe_int4_workspace_bytes(0, 8, 1408, 2048, 64) == 0
+    assert lib.moe_ffn_int4_workspace_bytes(6, 64, 2048, 1408, 64) >= 6 * 1408 * 2
     assert isinstance(Int4Tensor(torch.empty(3, 1, 1, 32, 4, dtype=torch.int32), torch.empty(3, 1, 1, 16), 16, 64,
                                  64).num_experts, int)
