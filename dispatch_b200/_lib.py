@@ -249,6 +249,8 @@ def check(rc: int, what: str) -> None:
 
 # ---------------------------------------------------------------- device state
 _status: dict[int, torch.Tensor] = {}
+# words that belong to a graph: made where the first call on a device is captured, zeroed by its replays
+_captured_status: dict[int, torch.Tensor] = {}
 _workspaces: dict[tuple[int, int, str], torch.Tensor] = {}
 
 
@@ -257,20 +259,22 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     s = _status.get(idx)
     if s is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the first call on a device must not be captured: make one before the capture")
-        s = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status[idx] = s
+        words = _captured_status if torch.cuda.is_current_stream_capturing() else _status
+        s = words.get(idx)
+        if s is None:
+            s = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+            words[idx] = s
     return s
 
 
 def check_device_status(device: torch.device) -> None:
     """Synchronises and raises MoeDeviceError if a kernel reported an error."""
-    s = status_word(device)
-    code = int(s.item())
-    if code != MOE_OK:
-        s.zero_()
-        raise MoeDeviceError(f"device reported: {lib().moe_status_string(code).decode()} ({code})")
+    eager = status_word(device)
+    for s in (eager, _captured_status.get(eager.device.index)):
+        code = MOE_OK if s is None else int(s.item())
+        if code != MOE_OK:
+            s.zero_()
+            raise MoeDeviceError(f"device reported: {lib().moe_status_string(code).decode()} ({code})")
 
 
 def workspace(device: torch.device, nbytes: int, tag: str) -> torch.Tensor:

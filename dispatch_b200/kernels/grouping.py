@@ -37,25 +37,35 @@ class TokenGrouping:
 class _DeviceGrouping(TokenGrouping):
     """A ``TokenGrouping`` whose int64 ``group_sizes`` and cast ``sorted_weight``
     are made from the kernels' int32 counts and f32 weights when they are first
-    read: two launches that a caller who only permutes and combines never needs."""
+    read: two launches that a caller who only permutes and combines never needs.
+    They are kept if made on the stream that made the grouping and not inside a
+    graph capture; a value made elsewhere is ordered only with its reader."""
+
+    def _keeps(self, v: torch.Tensor) -> bool:
+        return (not torch.cuda.is_current_stream_capturing()
+                and self.__dict__["_made_on"] == L.stream_ptr(v.device))
 
     @property
     def group_sizes(self) -> torch.Tensor:
         v = self.__dict__["_sizes"]
         if v.dtype != torch.int64:
-            v = self.__dict__["_sizes"] = v.to(torch.int64)
+            v = v.to(torch.int64)
+            if self._keeps(v):
+                self.__dict__["_sizes"] = v
         return v
 
     @group_sizes.setter
     def group_sizes(self, value: torch.Tensor) -> None:
         self.__dict__["_sizes"] = value
+        self.__dict__["_made_on"] = L.stream_ptr(value.device)
 
     @property
     def sorted_weight(self) -> torch.Tensor:
         v, dtype = self.__dict__["_sorted"]
         if v.dtype != dtype:
             v = v.to(dtype)
-            self.__dict__["_sorted"] = v, dtype
+            if self._keeps(v):
+                self.__dict__["_sorted"] = v, dtype
         return v
 
     @sorted_weight.setter

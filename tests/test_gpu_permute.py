@@ -230,6 +230,41 @@ def test_in_a_graph_and_refused_autograd_in_one() -> None:
     assert all(torch.equal(a, b) for a, b in zip(want, res))
 
 
+def test_sizes_first_read_inside_a_capture_or_on_another_stream() -> None:
+    idx = torch.randint(0, 4, (40, 2), device=DEV)
+    w = torch.rand(40, 2, device=DEV).to(BF16)
+    want = torch.bincount(idx.flatten(), minlength=4)
+    for where in ("graph", "stream"):
+        grouping = group_tokens_by_expert(idx, w, 4)
+        if where == "graph":
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):  # never replayed
+                grouping.group_sizes, grouping.sorted_weight
+        else:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                assert torch.equal(grouping.group_sizes, want)
+        first = grouping.group_sizes
+        assert torch.equal(first, want) and grouping.group_sizes is first
+        assert grouping.sorted_weight.dtype == BF16
+        assert torch.equal(grouping.sorted_weight.sort().values, w.flatten().sort().values)
+
+
+def test_first_call_on_a_device_captured(monkeypatch) -> None:
+    """Its status word belongs to the graph; an eager call before the first replay has its own."""
+    i, grouping, _ = make(33, 6, 64, 512, BF16)
+    want = permute_tokens(i["x"], grouping)
+    monkeypatch.setattr(L, "_status", {})
+    monkeypatch.setattr(L, "_captured_status", {})
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        xs = permute_tokens(i["x"], grouping)
+    assert torch.equal(permute_tokens(i["x"], grouping), want)
+    g.replay()
+    L.check_device_status(DEV)
+    assert torch.equal(xs, want) and L._status[0] is not L._captured_status[0]
+
+
 def test_refusals() -> None:
     i, grouping, _ = make(6, 2, 4, 64, BF16)
     with pytest.raises(ValueError, match="CUDA"):
