@@ -27,7 +27,6 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC,-O2",
     "-Xptxas", "-v",
-    "--split-compile", "0",  # optimise the kernels on all cores: half the build time
 ]
 
 
