@@ -1700,25 +1700,25 @@ struct RingShape {
   RingKernel kernel;
 };
 
-template <class T, int kTpr, int kNv>
+template <class T, int kTpr>
 RingShape ring_shape() {
-  using G = moe::norm::RingGroup<kTpr, kNv>;
+  using G = moe::norm::RingGroup<kTpr>;
   // once per kernel and process: the largest ring that it may be given
   static std::once_flag once;
   std::call_once(once, [] {
-    cudaFuncSetAttribute(moe::norm::norm_backward_ring_kernel<T, kTpr, kNv>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaFuncSetAttribute(moe::norm::norm_backward_ring_kernel<T, kTpr, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          kRingSmem);
   });
-  return {G::kThreads, G::kRpc, kTpr * kNv * 8, moe::norm::norm_backward_ring_kernel<T, kTpr, kNv>};
+  return {G::kThreads, G::kRpc, kTpr * 16, moe::norm::norm_backward_ring_kernel<T, kTpr, 2>};
 }
 
 template <class T>
 RingShape norm_backward_ring(int64_t v) {
-  if (v <= 64) return ring_shape<T, 32, 2>();
-  if (v <= 128) return ring_shape<T, 32, 4>();
-  if (v <= 256) return ring_shape<T, 64, 4>();
-  if (v <= 512) return ring_shape<T, 128, 4>();
-  return ring_shape<T, 256, 4>();
+  if (v <= 64) return ring_shape<T, 32>();
+  if (v <= 128) return ring_shape<T, 64>();
+  if (v <= 256) return ring_shape<T, 128>();
+  if (v <= 512) return ring_shape<T, 256>();
+  return ring_shape<T, 512>();
 }
 
 // The kernels with fixed types: `f(Types)` for the combination of one call, if

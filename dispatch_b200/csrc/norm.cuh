@@ -658,16 +658,11 @@ __global__ void __launch_bounds__(Group<kTpr>::kThreads) norm_backward_kernel(co
   if (p.part) write_sums<kTpr, kNv, G::kRpc>(p, acc, group, tx, join);
 }
 
-// The ring form: one CTA per SM, whose groups share a copy of the weights in
-// shared memory. A thread holds kNv vectors of its row, its column sums among
-// them, in the 64 kNv registers that 1024 / kNv threads leave each. Four
-// vectors on 256 threads beat two on 512 and one on 1024 (spilled): fewer
-// threads repeat a row's sums and addresses. Backward of 8192 x 2048 bf16, with
-// a channel gate / without: 66 / 52 us, 67 / 58, 100 / 79; 517 x 1000 f16 with a
-// full gate 11.4, 12.9, 14.7. Rows of at most 512 fit a warp with two.
-template <int kTpr, int kNv>
+// The ring form: one CTA of 512 threads per SM (128 registers a thread), whose
+// groups share a copy of the weights in shared memory.
+template <int kTpr>
 struct RingGroup {
-  static constexpr int kThreads = 1024 / kNv;
+  static constexpr int kThreads = 512;
   static constexpr int kRpc = kThreads / kTpr;
 };
 constexpr int kRingStages = 3;
@@ -689,9 +684,9 @@ struct RingParams {
 // latency) then never waits for HBM, and the arrays are read from shared
 // memory where they are used instead of living in registers.
 template <class T, int kTpr, int kNv>
-__global__ void __launch_bounds__(RingGroup<kTpr, kNv>::kThreads, 1)
+__global__ void __launch_bounds__(RingGroup<kTpr>::kThreads, 1)
     norm_backward_ring_kernel(const __grid_constant__ RingParams rp) {
-  using G = RingGroup<kTpr, kNv>;
+  using G = RingGroup<kTpr>;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ SumSlots<G::kRpc, kTpr / 32> slots;
   __shared__ uint64_t full[G::kRpc][kRingStages];
