@@ -145,8 +145,8 @@ struct Unit {
 //
 // Bounded by issue: per 256 weights one MMA per token tile and 9 (f16) or 11
 // (bf16) instructions that make its operand. 64 experts of 1408 x 2048 with
-// groups of 128: one token (6 experts) 7 us, 16 tokens 37 us (1.9 TB/s), 93
-// tokens 59 us; f16 2048 x 1408 with 16 tokens 29 us.
+// groups of 128: one token (6 experts) 7 us, 16 tokens 36 us, 93 tokens 59 us; f16
+// 2048 x 1408 with 16 tokens 28 us (50 busy experts, 2.7 TB/s).
 template <int kMt, int kNt, bool kSplit, bool kSwiglu, bool kF16, bool kG32>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNt)) int4_kernel(const __grid_constant__ Params p) {
   constexpr int kOutMt = kSwiglu ? kMt / 2 : kMt;  // output tiles of a unit

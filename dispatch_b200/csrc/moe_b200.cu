@@ -1969,12 +1969,12 @@ int log2_of(int64_t v) {
 
 // Which form multiplies M rows of E experts, by the rows of an average expert.
 // Measured on B200 (64 experts, 6 per token, 1408 x 2048; us; groups of 128 / 64 / 32):
-//   rows           1.5       6       8.7        12         24          48          64          96         128
-//   warp MMAs    37/37/37 44/42/46 59/57/80  60/58/81  90/85/116       -           -           -           -
-//   64-row tile  58/61/80 71/74/98 71/75/98 72/75/104 73/78/120  74/90/146  110/130/210 141/165/264 171/202/324
-//   128-row tile    -        -        -         -      91/134/236 98/153/264 104/163/281 107/182/326 169/297/553
-//   16 bits         -        -        -         -     154/157/161 155/158/162 156/159/163 158/161/165 180/183/186
-// (128 rows in 64-row tiles, 192 rows: 232 against 181 in 16 bits). Each scale group's sums pass
+//   rows         1.5         6           12          24          48          64          96          128
+//   warp MMAs    36/36/39    43/41/48    60/57/81    89/84/118   -           -           -           -
+//   64-row tile  58/66/80    71/76/99    71/76/105   72/80/120   74/91/147   110/133/212 142/170/266 178/208/326
+//   128-row tile 70/107/185  86/130/230  87/130/231  90/134/236  97/146/245  101/156/268 105/180/323 161/276/504
+//   16 bits      127/132/133 152/156/159 153/156/160 154/157/161 156/159/162 156/160/163 158/162/164 181/184/186
+// (192 rows, groups of 128: 236 in 64-row tiles, 224 in 128-row tiles, 181 in 16 bits). Each scale group's sums pass
 // through TMEM, so shorter groups cost the tiles more; the 128-row tile pays for groups of 128 on.
 enum class Int4Form { kWarp, kTile64, kTile128, k16Bit };
 Int4Form int4_form(int64_t M, int64_t E, int group) {
