@@ -99,6 +99,21 @@ int device_info(int* sms) {
   return MOE_OK;
 }
 
+// Lets a kernel be given `bytes` of dynamic shared memory on the current device:
+// once per kernel and device (`done`: one bit each; setting it twice is harmless).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel* kernel, int bytes, std::atomic<uint64_t>& done) {
+  static_assert(kMaxDevices <= 64, "one bit per device");
+  int dev = 0;
+  cudaError_t rc = cudaGetDevice(&dev);
+  if (rc != cudaSuccess) return rc;
+  const uint64_t bit = 1ull << (dev % kMaxDevices);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return rc;
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1698,18 +1713,15 @@ using RingKernel = void (*)(const moe::norm::RingParams);
 struct RingShape {
   int threads, rows_per_cta, columns;  // columns: a row's slot in a stage
   RingKernel kernel;
+  cudaError_t allowed;  // the largest ring's shared memory
 };
 
 template <class T, int kTpr>
 RingShape ring_shape() {
   using G = moe::norm::RingGroup<kTpr>;
-  // once per kernel and process: the largest ring that it may be given
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(moe::norm::norm_backward_ring_kernel<T, kTpr, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         kRingSmem);
-  });
-  return {G::kThreads, G::kRpc, kTpr * 16, moe::norm::norm_backward_ring_kernel<T, kTpr, 2>};
+  static std::atomic<uint64_t> done{0};
+  return {G::kThreads, G::kRpc, kTpr * 16, moe::norm::norm_backward_ring_kernel<T, kTpr, 2>,
+          allow_smem(moe::norm::norm_backward_ring_kernel<T, kTpr, 2>, kRingSmem, done)};
 }
 
 template <class T>
@@ -1896,6 +1908,7 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
     }
   }
   if (ring.kernel && stage_all + cols <= kRingSmem) {
+    CUDA_TRY(ring.allowed, "cudaFuncSetAttribute(norm backward)");
     rp.p = p;
     rp.status = status;
     const int64_t fit = (kRingSmem - cols) / stage_all;
@@ -2034,12 +2047,8 @@ int launch_int4(moe::int4::Params p, int64_t units, int sms, cudaStream_t stream
   stages = stages > moe::int4::kMaxStages ? moe::int4::kMaxStages : stages;
   p.stages = static_cast<int>(stages);
   const auto kernel = moe::int4::int4_kernel<kMt, kNt, kSplit, kSwiglu, kF16, kG32>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(int4)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(kernel, static_cast<int>(smem), done), "cudaFuncSetAttribute(int4)");
   const int64_t want = kSplit ? units : (units + moe::int4::kWarps - 1) / moe::int4::kWarps;
   const int64_t grid = want < per_sm * sms ? want : per_sm * sms;
   CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(moe::int4::kThreads),
@@ -2114,12 +2123,8 @@ int launch_int4_tile(const Int4Spec& s, int sms, int32_t* status, cudaStream_t s
   tp.tile_stages = static_cast<int>(fit > moe::int4::kTileStages ? moe::int4::kTileStages : fit);
   const size_t smem = moe::int4::tile_fixed_smem() + tp.tile_stages * stage + codes;
   const auto kernel = moe::int4::int4_tile_kernel<kSwiglu, kF16, kG32, kTok>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(int4 tile)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(kernel, static_cast<int>(kMaxDynSmem), done), "cudaFuncSetAttribute(int4 tile)");
   const int64_t tok = s.M / kTok + (s.E < s.M ? s.E : s.M);
   const int out_tiles = kSwiglu ? 4 : 8;
   const int64_t tiles = tok * ((tp.p.n16 + out_tiles - 1) / out_tiles);
