@@ -2128,6 +2128,7 @@ int launch_int4_tile(const Int4Spec& s, int sms, int32_t* status, cudaStream_t s
   const int64_t tok = s.M / kTok + (s.E < s.M ? s.E : s.M);
   const int out_tiles = kSwiglu ? 4 : 8;
   const int64_t tiles = tok * ((tp.p.n16 + out_tiles - 1) / out_tiles);
+  CHECK_ARG(tiles < (1ll << 31), "too many tiles: M=%lld rows of N=%lld", (long long)s.M, (long long)s.N);
   CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(tiles < sms ? tiles : sms)), dim3(Sh::kThreads), smem, stream,
                       tp),
            "int4_tile_kernel launch");
@@ -2175,7 +2176,9 @@ int run_int4(const Int4Spec& s, void* workspace, size_t workspace_bytes, int32_t
   rc = check_int4(s);
   if (rc || s.M == 0) return rc;
   const bool swiglu = s.data1 != nullptr;
-  const Int4Form form = int4_form(s.M, s.E, s.group);
+  Int4Form form = int4_form(s.M, s.E, s.group);
+  // Without room for 16-bit weights the codes themselves are multiplied, in the tiles that are faster for the group size.
+  if (form == Int4Form::k16Bit && !workspace) form = s.group >= 128 ? Int4Form::kTile128 : Int4Form::kTile64;
   if (form == Int4Form::kWarp)
     return swiglu ? run_int4_direct<true>(s, sms, status, stream) : run_int4_direct<false>(s, sms, status, stream);
   if (form == Int4Form::kTile64)
@@ -2184,8 +2187,7 @@ int run_int4(const Int4Spec& s, void* workspace, size_t workspace_bytes, int32_t
     return swiglu ? run_int4_tile<true, 128>(s, sms, status, stream) : run_int4_tile<false, 128>(s, sms, status, stream);
   const int projections = swiglu ? 2 : 1;
   const size_t need = int4_bytes(s.M, s.E, s.N, s.K, s.group, projections);
-  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= need, "workspace too small (%zu < %zu)",
-            workspace_bytes, need);
+  CHECK_ARG(aligned16(workspace) && workspace_bytes >= need, "workspace too small (%zu < %zu)", workspace_bytes, need);
   const int64_t chunk = int4_chunk(s.E, s.N, s.K, projections);
   void* w0 = workspace;
   void* w1 = static_cast<char*>(workspace) + need / projections;
@@ -2256,11 +2258,13 @@ int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, con
   if (R == 0) return MOE_OK;
   CHECK_ARG(gate && up && down, "null pointer");
   CHECK_ARG(I >= 8 && I % 8 == 0, "I=%lld must be a multiple of 8", (long long)I);
-  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= moe_ffn_int4_workspace_bytes(R, E, H, I, group),
-            "workspace too small");
   const size_t h_bytes = (static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255);
-  char* rest = static_cast<char*>(workspace) + h_bytes;
+  CHECK_ARG(workspace && aligned16(workspace) &&
+                (workspace_bytes >= moe_ffn_int4_workspace_bytes(R, E, H, I, group) || workspace_bytes == h_bytes),
+            "workspace too small");
+  // room for the intermediate rows alone: no weight is rounded
   const size_t rest_bytes = workspace_bytes - h_bytes;
+  char* rest = rest_bytes ? static_cast<char*>(workspace) + h_bytes : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Int4Spec s{};
   s.x = xs;

@@ -7,7 +7,7 @@ themselves are multiplied: they become 16-bit floats exactly on the way to the
 tensor cores (warp-level MMAs for a few rows, tcgen05 for more) and each column
 group's f32 sum is multiplied by its scale. Larger batches write the weights as
 16-bit ones, some experts at a time, for the 16-bit tcgen05 kernels (one
-rounding of code * scale per weight)."""
+rounding of code * scale per weight), unless the weights are marked ``exact``."""
 
 from __future__ import annotations
 
@@ -60,7 +60,9 @@ def grouped_matmul_int4(x: torch.Tensor, qweight: Int4Tensor, schedule: TileSche
     x = _aligned(x)
     offsets = device_offsets(schedule, dev)
     lib = L.lib()
-    ws = _workspace(lib.moe_int4_workspace_bytes(m, e, qweight.n, qweight.k, qweight.group_size), dev)
+    # without a workspace no weight is rounded
+    need = 0 if qweight.exact else lib.moe_int4_workspace_bytes(m, e, qweight.n, qweight.k, qweight.group_size)
+    ws = _workspace(need, dev)
     L.call(
         "grouped_matmul_int4", dev, lib.moe_grouped_gemm_int4,
         x.data_ptr(), L.dt(x), m, qweight.k, qweight.data.data_ptr(), qweight.scale.data_ptr(),
@@ -73,7 +75,7 @@ def grouped_matmul_int4(x: torch.Tensor, qweight: Int4Tensor, schedule: TileSche
 def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4StackedExpertWeights) -> torch.Tensor:
     """y = down(silu(gate(xs)) * up(xs)) per expert group of grouped rows, the
     offsets (E+1) int32 on the device; gate and up in one launch with SwiGLU
-    where they are joined."""
+    where they are joined. No weight is rounded if any of the three is ``exact``."""
     gate, up, down = weights.gate, weights.up, weights.down
     _check_activations(xs, gate)
     for q in (up, down):
@@ -90,7 +92,10 @@ def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4Stacke
     r, h, i, e = xs.shape[0], gate.k, gate.n, gate.num_experts
     y = torch.empty(r, h, dtype=xs.dtype, device=dev)
     lib = L.lib()
-    ws = _workspace(lib.moe_ffn_int4_workspace_bytes(r, e, h, i, gate.group_size), dev)
+    # room for the intermediate rows alone: no weight is rounded
+    exact = gate.exact or up.exact or down.exact
+    ws = _workspace((r * i * 2 + 255) // 256 * 256 if exact else
+                    lib.moe_ffn_int4_workspace_bytes(r, e, h, i, gate.group_size), dev)
     L.call(
         "expert_ffn_int4", dev, lib.moe_expert_ffn_int4,
         xs.data_ptr(), L.dt(xs), r, h, offsets.contiguous().data_ptr(), e, i, gate.data.data_ptr(),

@@ -45,10 +45,10 @@ def patch_moe_infer(model: torch.nn.Module, matmul=None, *, block_m: int = 16) -
 
 def patch_moe_infer_quantized(model: torch.nn.Module, matmul=None, *, block_m: int = 16,
                               scale_dtype: torch.dtype = torch.float32, bits: int = 8,
-                              group_size: int = 128) -> int:
+                              group_size: int = 128, exact: bool = False) -> int:
     """Quantises each layer's stacked weights once, to int8 per channel or
-    (``bits`` 4) to int4 in groups of ``group_size`` columns, frees the
-    originals, and installs the quantised path."""
+    (``bits`` 4) to int4 in groups of ``group_size`` columns (``exact``: as in
+    ``Int4Tensor``), frees the originals, and installs the quantised path."""
     if bits not in (4, 8):
         raise ValueError(f"bits must be 4 or 8, got {bits}")
     model.eval()
@@ -56,7 +56,8 @@ def patch_moe_infer_quantized(model: torch.nn.Module, matmul=None, *, block_m: i
     for module, experts in _iter_validated_moe_layers(model):
         stacked = stack_expert_weights(experts)
         if bits == 4:
-            qweights = quantize_stacked_weights_int4(stacked, group_size=group_size, scale_dtype=scale_dtype)
+            qweights = quantize_stacked_weights_int4(stacked, group_size=group_size, scale_dtype=scale_dtype,
+                                                     exact=exact)
         else:
             qweights = quantize_stacked_weights(stacked, scale_dtype=scale_dtype)
         del stacked

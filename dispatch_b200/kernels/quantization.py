@@ -129,13 +129,19 @@ class Int4Tensor:
     """(E, N, K) weights as 4-bit codes -8..7 and one scale per row and group
     of ``group_size`` columns, laid out once for the product's kernels
     (``include/moe_b200.h``): ``data`` (E, ceil(N/16), ceil(K/64), 32, 4) int32,
-    ``scale`` (E, ceil(N/16), ceil(K/group_size), 16) f32, bf16 or f16."""
+    ``scale`` (E, ceil(N/16), ceil(K/group_size), 16) f32, bf16 or f16.
+
+    Batches of more than 128 rows per expert on average (48 for groups below
+    128) round each weight code * scale once to the activation type, in f16
+    within f16's range, for the 16-bit kernels. ``exact``: no batch rounds a
+    weight; the codes are multiplied and the scales act in f32 at any size."""
 
     data: torch.Tensor
     scale: torch.Tensor
     n: int
     k: int
     group_size: int
+    exact: bool = False
 
     @property
     def num_experts(self) -> int:
@@ -180,7 +186,7 @@ def _check_int4(q: Int4Tensor) -> None:
 
 
 def quantize_groupwise_int4(weight: torch.Tensor, *, group_size: int = 128,
-                            scale_dtype: torch.dtype = torch.float32) -> Int4Tensor:
+                            scale_dtype: torch.dtype = torch.float32, exact: bool = False) -> Int4Tensor:
     """Per row and group of columns: scale = absmax / 7 in f32 (1.0 for a group
     of zeros) rounded to ``scale_dtype``, code = clamp(round_half_even(w /
     scale), -8, 7). weight (E, N, K); a last group of fewer columns is fine."""
@@ -196,10 +202,10 @@ def quantize_groupwise_int4(weight: torch.Tensor, *, group_size: int = 128,
     scale = torch.empty(e, -(-n // 16), -(-k // group_size), 16, dtype=scale_dtype, device=dev)
     L.call("quantize_groupwise_int4", dev, L.lib().moe_quantize_int4, w.data_ptr(), L.dt(w), e, n, k, group_size,
            data.data_ptr(), scale.data_ptr(), L.dt(scale), L.stream_ptr(dev))
-    return Int4Tensor(data, scale, n, k, group_size)
+    return Int4Tensor(data, scale, n, k, group_size, exact)
 
 
-def pack_int4(codes: torch.Tensor, scale: torch.Tensor, group_size: int) -> Int4Tensor:
+def pack_int4(codes: torch.Tensor, scale: torch.Tensor, group_size: int, *, exact: bool = False) -> Int4Tensor:
     """Lays out codes (E, N, K), integers -8..7, and their scales (E, N,
     ceil(K/group_size)): for weights quantised elsewhere. Runs once per weight,
     on the codes' device (CPU included)."""
@@ -217,7 +223,7 @@ def pack_int4(codes: torch.Tensor, scale: torch.Tensor, group_size: int) -> Int4
     data = (u[..., 0] | (u[..., 1] << 4)).reshape(e, n16, kb, 32, 16).contiguous().view(torch.int32)
     s = torch.nn.functional.pad(scale, (0, 0, 0, -n % 16), value=1.0)
     s = s.view(e, n16, 16, -1).transpose(2, 3).contiguous()
-    return Int4Tensor(data, s, n, k, group_size)
+    return Int4Tensor(data, s, n, k, group_size, exact)
 
 
 def unpack_int4(q: Int4Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -240,9 +246,10 @@ def dequantize_int4(q: Int4Tensor) -> torch.Tensor:
 
 
 def quantize_stacked_weights_int4(weights, *, group_size: int = 128,
-                                  scale_dtype: torch.dtype = torch.float32) -> Int4StackedExpertWeights:
+                                  scale_dtype: torch.dtype = torch.float32,
+                                  exact: bool = False) -> Int4StackedExpertWeights:
     """Each projection of a ``StackedExpertWeights`` in 4 bits."""
     return Int4StackedExpertWeights(*(
-        quantize_groupwise_int4(w, group_size=group_size, scale_dtype=scale_dtype)
+        quantize_groupwise_int4(w, group_size=group_size, scale_dtype=scale_dtype, exact=exact)
         for w in (weights.gate, weights.up, weights.down)
     ))

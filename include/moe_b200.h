@@ -397,7 +397,8 @@ int moe_norm_gate_residual_backward(const MoeNormDesc* d, const void* d_out, int
  * are written as code * scale rounded to x's type and multiplied on the 16-bit
  * tcgen05 kernels; f16 then holds them in f16's range, as it does f16 weights.
  * workspace: moe_int4_workspace_bytes (0 where none is needed), 16-byte
- * aligned, no initialisation. x (M, K) and out (M, ldo) bf16 or f16.
+ * aligned, no initialisation. NULL: no weight is rounded at any batch size, at
+ * the tile kernel's speed. x (M, K) and out (M, ldo) bf16 or f16.
  */
 #define MOE_INT4_EXACT_ROWS(group) ((group) >= 128 ? 128 : 48)
 size_t moe_int4_workspace_bytes(int64_t M, int64_t E, int64_t N, int64_t K, int group);
@@ -408,7 +409,8 @@ int moe_grouped_gemm_int4(const void* x, int x_dtype, int64_t M, int64_t K, cons
  * The expert FFN over grouped rows with 4-bit weights, as moe_expert_ffn:
  * y = (silu(xs gate^T) * (xs up^T)) down^T, gate/up (E, I, H) and down
  * (E, H, I) laid out, one group size and scale type for the three. The
- * intermediate rows are in xs' type (in the workspace), SwiGLU in f32.
+ * intermediate rows are in xs' type (in the workspace), SwiGLU in f32. A
+ * workspace of R * I * 2 bytes rounded up to 256, no more: no weight is rounded.
  */
 size_t moe_ffn_int4_workspace_bytes(int64_t R, int64_t E, int64_t H, int64_t I, int group);
 int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, const int32_t* offsets, int64_t E,
