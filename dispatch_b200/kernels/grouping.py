@@ -34,45 +34,6 @@ class TokenGrouping:
     top_k: int
 
 
-class _DeviceGrouping(TokenGrouping):
-    """A ``TokenGrouping`` whose int64 ``group_sizes`` and cast ``sorted_weight``
-    are made from the kernels' int32 counts and f32 weights when they are first
-    read: two launches that a caller who only permutes and combines never needs.
-    They are kept if made on the stream that made the grouping and not inside a
-    graph capture; a value made elsewhere is ordered only with its reader."""
-
-    def _keeps(self, v: torch.Tensor) -> bool:
-        return (not torch.cuda.is_current_stream_capturing()
-                and self.__dict__["_made_on"] == L.stream_ptr(v.device))
-
-    @property
-    def group_sizes(self) -> torch.Tensor:
-        v = self.__dict__["_sizes"]
-        if v.dtype != torch.int64:
-            v = v.to(torch.int64)
-            if self._keeps(v):
-                self.__dict__["_sizes"] = v
-        return v
-
-    @group_sizes.setter
-    def group_sizes(self, value: torch.Tensor) -> None:
-        self.__dict__["_sizes"] = value
-        self.__dict__["_made_on"] = L.stream_ptr(value.device)
-
-    @property
-    def sorted_weight(self) -> torch.Tensor:
-        v, dtype = self.__dict__["_sorted"]
-        if v.dtype != dtype:
-            v = v.to(dtype)
-            if self._keeps(v):
-                self.__dict__["_sorted"] = v, dtype
-        return v
-
-    @sorted_weight.setter
-    def sorted_weight(self, value) -> None:
-        self.__dict__["_sorted"] = value if isinstance(value, tuple) else (value, value.dtype)
-
-
 def _group(topk_idx: torch.Tensor, topk_weight: torch.Tensor | None, n_experts: int,
            x: torch.Tensor | None = None, xs_dtype: torch.dtype | None = None,
            want_sorted: bool = True):
@@ -115,12 +76,12 @@ def group_tokens_by_expert(
             f"topk_idx.shape {tuple(topk_idx.shape)} != topk_weight.shape {tuple(topk_weight.shape)}"
         )
     counts, offsets, pos, sti, sw, w, _ = _group(topk_idx, topk_weight, n_routed_experts)
-    if torch.cuda.is_current_stream_capturing():  # part of the graph, or replays would not update them
-        counts, sw = counts.to(torch.int64), sw.to(topk_weight.dtype)
-    return _DeviceGrouping(
+    # made here, on the grouping's own stream: a caller who reads them elsewhere
+    # can then protect them with record_stream, or keep them for a captured graph
+    return TokenGrouping(
         sorted_token_idx=sti,
-        sorted_weight=(sw, topk_weight.dtype),
-        group_sizes=counts,
+        sorted_weight=sw.to(topk_weight.dtype),
+        group_sizes=counts.to(torch.int64),
         offsets=offsets,
         pos=pos,
         flat_weight=w.reshape(-1),

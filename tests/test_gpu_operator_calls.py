@@ -1,0 +1,76 @@
+"""Calls of the operators around the layer as programs make them: graphs that
+are replayed in any order, other streams and devices, empty batches."""
+
+from __future__ import annotations
+
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover - collected on CPU hosts too
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+
+from dispatch_b200 import _lib as L  # noqa: E402
+from dispatch_b200.kernels.grouping import group_tokens_by_expert  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _device_status_clean():
+    yield
+    L.check_device_status(DEV)
+
+
+def grouped(t=33, k=6, e=64, h=512, dev=DEV, wdtype=F32):
+    g = torch.Generator().manual_seed(t)
+    idx = torch.multinomial(torch.ones(t, e), k, generator=g).to(dev)
+    w = torch.rand(t, k, generator=g).to(dev, wdtype)
+    x = torch.randn(t, h, generator=g).to(dev, BF16)
+    y = torch.randn(t * k, h, generator=g).to(dev, BF16)
+    return x, y, w, idx, group_tokens_by_expert(idx, w, e)
+
+
+# ------------------------------------------------------------------ streams
+@pytest.mark.parametrize("wdtype", [F32, BF16])
+def test_sizes_belong_to_the_stream_that_made_them(wdtype) -> None:
+    """What a grouping holds is made when it is: reading it elsewhere launches
+    nothing, so record_stream of what was read protects the memory itself."""
+    _, _, w, idx, grouping = grouped(wdtype=wdtype)
+    want = torch.bincount(idx.flatten(), minlength=64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = grouping.group_sizes, grouping.sorted_weight
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):  # never replayed
+        captured = grouping.group_sizes, grouping.sorted_weight
+    for a, b, c in zip(there, captured, (grouping.group_sizes, grouping.sorted_weight)):
+        assert a is b and b is c
+    assert there[0].dtype == torch.int64 and there[1].dtype == wdtype
+    assert torch.equal(there[0], want)
+    order = torch.sort(idx.flatten(), stable=True).indices
+    assert torch.equal(there[1], w.flatten()[order])
+
+
+def test_a_dropped_groupings_sizes_read_on_another_stream() -> None:
+    want = torch.bincount(grouped()[3].flatten(), minlength=64)
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        grouping = grouped()[4]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000)
+            sizes = grouping.group_sizes
+            sizes.record_stream(side)
+            del grouping
+            got = sizes + 0
+            del sizes
+        for _ in range(8):  # what the making stream allocates next
+            torch.full((64,), -1, device=DEV)
+            torch.full((64,), -1, device=DEV, dtype=torch.int32)
+        side.synchronize()
+        assert torch.equal(got, want)
