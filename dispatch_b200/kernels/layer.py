@@ -53,13 +53,16 @@ def moe_layer_forward(
     """x (T, H) bf16/f16 (or f32 with bf16 weights and no shared expert);
     router_weight (E, H) bf16/f32; ``topk`` = (idx int32 (T,k), w f32 (T,k))
     skips the router (the moe_infer contract)."""
+    if topk is not None and not (topk[0].shape == topk[1].shape == (x.shape[0], router.top_k)):
+        raise ValueError(f"topk of shapes {tuple(topk[0].shape)} and {tuple(topk[1].shape)}, expected "
+                         f"({x.shape[0]}, {router.top_k}) both")
     if isinstance(weights, Int4StackedExpertWeights):
         return _layer_int4(x, router_weight, weights, router, shared, e_score_bias, topk, out_dtype)
     quant = isinstance(weights, QuantizedStackedExpertWeights)
     g = weights.gate.data if quant else weights.gate
     u = weights.up.data if quant else weights.up
     dn = weights.down.data if quant else weights.down
-    dev = L.require_cuda(x, router_weight, g, u, dn, e_score_bias, what="moe_layer_forward")
+    dev = L.require_cuda(x, router_weight, g, u, dn, e_score_bias, *(topk or ()), what="moe_layer_forward")
     act = act_dtype_for(x, weights)
     t, h = x.shape
     e, i, _ = g.shape

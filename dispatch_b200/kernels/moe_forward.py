@@ -209,6 +209,8 @@ def _routed_forward(x, topk_idx, topk_weight, weights, shared: SharedExpertWeigh
         raise ValueError(
             f"topk_idx.shape {tuple(topk_idx.shape)} != topk_weight.shape {tuple(topk_weight.shape)}"
         )
+    if x.shape[0] < topk_idx.shape[0]:
+        raise ValueError(f"x has {x.shape[0]} rows, topk_idx.shape is {tuple(topk_idx.shape)}")
     act = act_dtype_for(x, weights)
     if act not in (torch.bfloat16, torch.float16):
         raise ValueError(f"dtype mismatch: expert weights must be bf16/f16 (or int8), got {act}")

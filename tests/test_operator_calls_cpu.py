@@ -3,10 +3,17 @@ let through, before anything runs on a GPU."""
 
 from __future__ import annotations
 
+import pytest
 import torch
 
-from dispatch_b200.kernels.moe_forward import StackedExpertWeights
-from dispatch_b200.kernels.quantization import Int4StackedExpertWeights, Int4Tensor, pack_int4
+from dispatch_b200.kernels.layer import RouterConfig, moe_block_forward, moe_layer_forward
+from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed
+from dispatch_b200.kernels.quantization import (
+    Int4StackedExpertWeights,
+    Int4Tensor,
+    grouped_moe_routed_quantized,
+    pack_int4,
+)
 
 BF16 = torch.bfloat16
 T, K, E, H, I = 6, 2, 4, 64, 32
@@ -25,6 +32,27 @@ def weights(kind):
 
 def topk(t=T, k=K):
     return torch.zeros(t, k, dtype=torch.int32), torch.ones(t, k)
+
+
+# ------------------------------------------------------------------ the caller's top-k
+@pytest.mark.parametrize("kind", ["int4", "bf16"])
+@pytest.mark.parametrize("pair", [topk(T, K - 1), topk(T, K + 1), topk(T - 1, K), topk(T + 1, K), topk(K, T),
+                                  (topk()[0], topk(T, K - 1)[1]), (topk()[0].flatten(), topk()[1].flatten())])
+def test_topk_of_another_shape_is_refused(kind, pair) -> None:
+    x = torch.zeros(T, H, dtype=BF16)
+    with pytest.raises(ValueError, match="topk"):
+        moe_layer_forward(x, None, weights(kind), RouterConfig(top_k=K), topk=pair)
+    with pytest.raises(ValueError, match="topk"):
+        moe_block_forward(x, None, None, weights(kind), RouterConfig(top_k=K), normed=x, topk=pair)
+    with pytest.raises(ValueError, match="CUDA"):  # the right one goes on to the device check
+        moe_layer_forward(x, None, weights(kind), RouterConfig(top_k=K), topk=topk())
+
+
+@pytest.mark.parametrize("kind", ["int4", "bf16"])
+def test_fewer_rows_than_the_topk_names_are_refused(kind) -> None:
+    call = grouped_moe_routed_quantized if kind == "int4" else grouped_moe_routed
+    with pytest.raises(ValueError, match="topk_idx"):
+        call(torch.zeros(T - 1, H, dtype=BF16), *topk(), weights(kind))
 
 
 # ------------------------------------------------------------------ weights
