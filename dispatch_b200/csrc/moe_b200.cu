@@ -2020,7 +2020,7 @@ int check_int4(const Int4Spec& s) {
   CHECK_ARG(s.K >= 8 && s.K % 8 == 0 && s.K < (1 << 30), "K mismatch: K=%lld must be a multiple of 8", (long long)s.K);
   CHECK_ARG(s.N >= 1 && s.N < (1 << 30) && s.M >= 0 && s.M < (1ll << 31) && s.ldo >= s.N, "bad M/N/ldo");
   if (s.M == 0) return MOE_OK;
-  CHECK_ARG(s.x && s.data0 && s.scale0 && s.offsets && s.out, "null pointer");
+  CHECK_ARG(s.x && s.data0 && s.scale0 && (!s.data1 || s.scale1) && s.offsets && s.out, "null pointer");
   CHECK_ARG(aligned16(s.x) && aligned16(s.data0) && aligned16(s.scale0) && aligned16(s.data1) && aligned16(s.scale1),
             "x, weights and scales must be 16-byte aligned");
   return MOE_OK;
@@ -2256,7 +2256,8 @@ int moe_expert_ffn_int4(const void* xs, int act_dtype, int64_t R, int64_t H, con
                         const void* down, const void* down_scale, int scale_dtype, int group, void* y,
                         void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   if (R == 0) return MOE_OK;
-  CHECK_ARG(gate && up && down, "null pointer");
+  // all of them before the first product is launched
+  CHECK_ARG(xs && offsets && y && gate && up && down && gate_scale && up_scale && down_scale, "null pointer");
   CHECK_ARG(I >= 8 && I % 8 == 0, "I=%lld must be a multiple of 8", (long long)I);
   const size_t h_bytes = (static_cast<size_t>(R) * I * 2 + 255) & ~size_t(255);
   CHECK_ARG(workspace && aligned16(workspace) &&

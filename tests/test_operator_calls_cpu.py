@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from dispatch_b200 import _lib as L
 from dispatch_b200.kernels.layer import RouterConfig, moe_block_forward, moe_layer_forward
 from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed
 from dispatch_b200.kernels.quantization import (
@@ -53,6 +54,18 @@ def test_fewer_rows_than_the_topk_names_are_refused(kind) -> None:
     call = grouped_moe_routed_quantized if kind == "int4" else grouped_moe_routed
     with pytest.raises(ValueError, match="topk_idx"):
         call(torch.zeros(T - 1, H, dtype=BF16), *topk(), weights(kind))
+
+
+# ------------------------------------------------------------------ arguments of the C entries
+@pytest.mark.parametrize("missing", ["gate_scale", "up_scale", "down_scale"])
+def test_ffn_without_a_scale_is_refused(missing) -> None:
+    """Before any launch, and before the device is looked at. The addresses are never read."""
+    lib, at = L.lib(), 4096
+    scale = {n: None if n == missing else at for n in ("gate_scale", "up_scale", "down_scale")}
+    rc = lib.moe_expert_ffn_int4(at, L.DT_BF16, 8, H, at, E, I, at, scale["gate_scale"], at, scale["up_scale"], at,
+                                 scale["down_scale"], L.DT_F32, 32, at, at,
+                                 lib.moe_ffn_int4_workspace_bytes(8, E, H, I, 32), None, None)
+    assert rc == L.MOE_ERR_INVALID_ARG and b"null" in lib.moe_last_error()
 
 
 # ------------------------------------------------------------------ weights
