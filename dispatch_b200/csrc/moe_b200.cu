@@ -288,13 +288,9 @@ int check_seg(const SegSpec& sp, int act_dtype) {
 template <bool kInt8>
 int launch_gemm(const moe::gemm::Params& p, int sms, cudaStream_t stream) {
   constexpr size_t smem = moe::gemm::smem_bytes<kInt8>();
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(moe::gemm::grouped_gemm_kernel<kInt8>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(gemm)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(moe::gemm::grouped_gemm_kernel<kInt8>, static_cast<int>(smem), done),
+           "cudaFuncSetAttribute(gemm)");
   CUDA_TRY(launch_pdl(moe::gemm::grouped_gemm_kernel<kInt8>, dim3(sms), dim3(moe::gemm::Config<kInt8>::kThreads),
                       smem, stream, p),
            "grouped_gemm_kernel launch");
@@ -358,13 +354,9 @@ int run_gemm(const SegSpec* specs_in, int nseg, int act_dtype, int32_t* status, 
 int launch_pair(const moe::gemm::Params& p, int grid, cudaStream_t stream) {
   constexpr size_t smem = moe::gemm::pair_smem_bytes();
   static_assert(smem <= 232448, "shared memory of the CTA-pair kernel");
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(moe::gemm::grouped_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(smem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(pair gemm)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(moe::gemm::grouped_gemm_pair_kernel, static_cast<int>(smem), done),
+           "cudaFuncSetAttribute(pair gemm)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(moe::gemm::kPairThreads);
@@ -426,13 +418,9 @@ template <int kWarps, bool kInt8>
 int launch_warp(const moe::gemm::WarpParams& wp, int grid, cudaStream_t stream) {
   constexpr size_t smem = moe::gemm::warp_smem_bytes<kWarps>();
   static_assert(2 * (smem + 1024) <= 233472, "two warp-MMA CTAs per SM");
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(moe::gemm::grouped_gemm_warp_kernel<kWarps, kInt8>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(warp gemm)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(moe::gemm::grouped_gemm_warp_kernel<kWarps, kInt8>, static_cast<int>(smem), done),
+           "cudaFuncSetAttribute(warp gemm)");
   CUDA_TRY(launch_pdl(moe::gemm::grouped_gemm_warp_kernel<kWarps, kInt8>, dim3(grid),
                       dim3(moe::gemm::WarpConfig<kWarps>::kThreads), smem, stream, wp),
            "grouped_gemm_warp_kernel launch");
@@ -509,13 +497,9 @@ constexpr size_t kMaxDynSmem = 232448;
 
 template <bool kInt8>
 int launch_stream(const moe::gemm::StreamParams& sp, int grid, size_t smem, cudaStream_t stream) {
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [] {
-    attr_err = cudaFuncSetAttribute(moe::gemm::grouped_gemm_stream_kernel<kInt8>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem));
-  });
-  if (attr_err != cudaSuccess) return cuda_fail(attr_err, "cudaFuncSetAttribute(stream gemm)");
+  static std::atomic<uint64_t> done{0};
+  CUDA_TRY(allow_smem(moe::gemm::grouped_gemm_stream_kernel<kInt8>, static_cast<int>(kMaxDynSmem), done),
+           "cudaFuncSetAttribute(stream gemm)");
   CUDA_TRY(launch_pdl(moe::gemm::grouped_gemm_stream_kernel<kInt8>, dim3(grid),
                       dim3(moe::gemm::StreamConfig<kInt8>::kThreads), smem, stream, sp),
            "grouped_gemm_stream_kernel launch");
@@ -752,16 +736,12 @@ int moe_route(const void* x, int x_dtype, const void* router_w, int w_dtype, con
   p.scaling = routed_scaling;
   p.tb = route_tb(H, p.E, logits_in == nullptr);
   const size_t smem = static_cast<size_t>(p.tb) * (p.E + (logits_in ? 0 : H)) * sizeof(float);
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(moe::route::route_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    cudaFuncSetAttribute(moe::route::route_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    cudaFuncSetAttribute(moe::route::route_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  });
   const int64_t grid = (T + p.tb - 1) / p.tb;
   // experts per lane in the selection: the fewest that cover E
   auto kernel = p.E <= 64 ? moe::route::route_kernel<2> : p.E <= 128 ? moe::route::route_kernel<4>
                                                                         : moe::route::route_kernel<8>;
+  static std::array<std::atomic<uint64_t>, 3> done{};
+  CUDA_TRY(allow_smem(kernel, 160 * 1024, done[p.E <= 64 ? 0 : p.E <= 128 ? 1 : 2]), "cudaFuncSetAttribute(route)");
   CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(moe::route::kThreads), smem, s, p),
            "route_kernel launch");
   return MOE_OK;

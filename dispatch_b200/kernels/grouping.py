@@ -57,13 +57,13 @@ def _group(topk_idx: torch.Tensor, topk_weight: torch.Tensor | None, n_experts: 
     lib = L.lib()
     nbytes = lib.moe_group_workspace_bytes(t, k, n_experts)
     ws = L.workspace(dev, nbytes, "group")
-    rc = lib.moe_group_tokens(
+    L.call(
+        "group_tokens_by_expert", dev, lib.moe_group_tokens,
         idx.data_ptr(), L.dt(idx), L.ptr(w), t, k, n_experts, counts.data_ptr(), offsets.data_ptr(),
         pos.data_ptr(), L.ptr(sti), L.ptr(sw),
         L.ptr(x), L.dt(x) if x is not None else 0, h, L.ptr(xs), L.dt(xs_dtype) if xs is not None else 0,
         ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
-    L.check(rc, "group_tokens_by_expert")
     return counts, offsets, pos, sti, sw, w, xs
 
 
@@ -98,11 +98,11 @@ def combine(y: torch.Tensor, pos: torch.Tensor, flat_weight: torch.Tensor, num_t
     ys = None if y_shared is None else y_shared.contiguous()
     if ys is not None and ys.dtype != y.dtype:
         ys = ys.to(y.dtype)
-    rc = L.lib().moe_combine(
+    L.call(
+        "ungroup_and_combine", dev, L.lib().moe_combine,
         y.contiguous().data_ptr(), L.dt(y), pos.data_ptr(), flat_weight.contiguous().data_ptr(), num_tokens,
         top_k, h, L.ptr(ys), out.data_ptr(), L.dt(out), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
-    L.check(rc, "ungroup_and_combine")
     return out
 
 

@@ -99,7 +99,8 @@ def moe_layer_forward(
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
     rw = None if router_weight is None else router_weight.contiguous()
     sc = (weights.gate.scale, weights.up.scale, weights.down.scale) if quant else (None, None, None)
-    rc = lib.moe_layer_forward(
+    L.call(
+        "moe_layer_forward", dev, lib.moe_layer_forward,
         ctypes.byref(desc), x.data_ptr(), L.ptr(rw), L.ptr(e_score_bias),
         L.ptr(idx_in), L.ptr(w_in),
         g.contiguous().data_ptr(), u.contiguous().data_ptr(), dn.contiguous().data_ptr(),
@@ -110,7 +111,6 @@ def moe_layer_forward(
         counts.data_ptr(), offsets.data_ptr(), ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(),
         L.stream_ptr(dev),
     )
-    L.check(rc, "moe_layer_forward")
     return LayerOutput(out, idx, wts, counts, offsets)
 
 
@@ -215,7 +215,8 @@ def route(
     bias = None if e_score_bias is None else e_score_bias.contiguous().float()
     lib = L.lib()
     ws = None if logits is not None else L.workspace(dev, lib.moe_route_workspace_bytes(t, e), "route")
-    rc = lib.moe_route(
+    L.call(
+        "route", dev, lib.moe_route,
         None if logits is not None else x.data_ptr(), 0 if logits is not None else L.dt(x),
         None if logits is not None else router_weight.data_ptr(), 0 if logits is not None else L.dt(router_weight),
         L.ptr(logits), t, h, e, k,
@@ -224,7 +225,6 @@ def route(
         idx.data_ptr(), w.data_ptr(), L.ptr(lg), L.ptr(ws), 0 if ws is None else ws.numel(),
         L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
-    L.check(rc, "route")
     return (idx, w, lg) if return_logits else (idx, w)
 
 

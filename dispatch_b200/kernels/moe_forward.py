@@ -148,7 +148,8 @@ def expert_ffn(xs: torch.Tensor, offsets: torch.Tensor, weights, shared: SharedE
     nbytes = lib.moe_ffn_workspace_bytes(r, i, t_sh, i_sh)
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
     sc = (weights.gate.scale, weights.up.scale, weights.down.scale) if quant else (None, None, None)
-    rc = lib.moe_expert_ffn_grouped(
+    L.call(
+        "expert_ffn", dev, lib.moe_expert_ffn_grouped,
         3, xs.data_ptr(), L.dt(act), r, h, offsets.data_ptr(), e, e,
         L.ptr(gather_rows), xs.shape[0] if gather_rows is not None else 0, i,
         g.contiguous().data_ptr(), u.contiguous().data_ptr(), d.contiguous().data_ptr(),
@@ -160,7 +161,6 @@ def expert_ffn(xs: torch.Tensor, offsets: torch.Tensor, weights, shared: SharedE
         L.ptr(None if shared is None else shared.down.contiguous()),
         y.data_ptr(), L.ptr(ys), ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
-    L.check(rc, "expert_ffn")
     return y, ys
 
 

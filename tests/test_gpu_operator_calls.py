@@ -14,7 +14,19 @@ if not torch.cuda.is_available():  # pragma: no cover - collected on CPU hosts t
 
 
 from dispatch_b200 import _lib as L  # noqa: E402
-from dispatch_b200.kernels.grouping import group_tokens_by_expert  # noqa: E402
+from dispatch_b200.kernels.block import norm_gate_residual, norm_gate_residual_backward  # noqa: E402
+from dispatch_b200.kernels.grouped_gemm_int4 import grouped_matmul_int4  # noqa: E402
+from dispatch_b200.kernels.grouping import (  # noqa: E402
+    combine_tokens,
+    combine_tokens_backward,
+    group_tokens_by_expert,
+    permute_tokens,
+    permute_tokens_backward,
+)
+from dispatch_b200.kernels.layer import RouterConfig, moe_layer_forward  # noqa: E402
+from dispatch_b200.kernels.moe_forward import StackedExpertWeights  # noqa: E402
+from dispatch_b200.kernels.quantization import pack_int4, quantize_stacked_weights_int4  # noqa: E402
+from dispatch_b200.kernels.tile_schedule import build_tile_schedule  # noqa: E402
 
 DEV = torch.device("cuda", 0)
 BF16, F32 = torch.bfloat16, torch.float32
@@ -74,3 +86,33 @@ def test_a_dropped_groupings_sizes_read_on_another_stream() -> None:
             torch.full((64,), -1, device=DEV, dtype=torch.int32)
         side.synchronize()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ devices
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_every_form_on_a_second_device() -> None:
+    """The first device's calls come first, and it stays the current one."""
+    results = []
+    for dev in (torch.device("cuda", 0), torch.device("cuda", 1)):
+        got = []
+        g = torch.Generator().manual_seed(0)
+        codes = torch.randint(-8, 8, (2, 48, 256), generator=g).to(torch.int8).to(dev)
+        for group in (32, 128):
+            q = pack_int4(codes, torch.ones(2, 48, 256 // group, device=dev) / 16, group)
+            for rows in (3, 20, 60, 100, 300):
+                x = torch.randn(2 * rows, 256, generator=g).to(dev, BF16)
+                got.append(grouped_matmul_int4(x, q, build_tile_schedule(torch.tensor([rows, rows]), 16)))
+        x, y, w, idx, grouping = grouped(dev=dev)
+        got += [permute_tokens(x, grouping), combine_tokens(y, grouping, w), permute_tokens_backward(y, grouping),
+                *combine_tokens_backward(x, y, grouping, w)]
+        weight = torch.ones(512, device=dev)
+        got += [*norm_gate_residual(x, x, weight, weight), *norm_gate_residual_backward(x, x, x, x, weight, weight)[:4]]
+        stacked = StackedExpertWeights(*((torch.randn(64, a, b, generator=g) / 16).to(dev, BF16)
+                                         for a, b in ((48, 512), (48, 512), (512, 48))))
+        router_weight = torch.randn(64, 512, generator=g).to(dev, BF16)
+        for weights in (stacked, quantize_stacked_weights_int4(stacked, group_size=64)):
+            got.append(moe_layer_forward(x, router_weight, weights, RouterConfig(top_k=6)).out)
+            got.append(moe_layer_forward(x, None, weights, RouterConfig(top_k=6), topk=(idx, w)).out)
+        results.append([t.cpu() for t in got])
+        L.check_device_status(dev)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
