@@ -88,7 +88,7 @@ def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4Stacke
         raise ValueError("offsets must be (E+1,) int32")
     dev = L.require_cuda(xs, offsets, *(t for q in (gate, up, down) for t in (q.data, q.scale)),
                          what="the B200 int4 expert FFN")
-    xs = _aligned(xs)
+    xs, offsets = _aligned(xs), offsets.contiguous()
     r, h, i, e = xs.shape[0], gate.k, gate.n, gate.num_experts
     y = torch.empty(r, h, dtype=xs.dtype, device=dev)
     lib = L.lib()
@@ -98,7 +98,7 @@ def expert_ffn_int4(xs: torch.Tensor, offsets: torch.Tensor, weights: Int4Stacke
                     lib.moe_ffn_int4_workspace_bytes(r, e, h, i, gate.group_size), dev)
     L.call(
         "expert_ffn_int4", dev, lib.moe_expert_ffn_int4,
-        xs.data_ptr(), L.dt(xs), r, h, offsets.contiguous().data_ptr(), e, i, gate.data.data_ptr(),
+        xs.data_ptr(), L.dt(xs), r, h, offsets.data_ptr(), e, i, gate.data.data_ptr(),
         gate.scale.data_ptr(), up.data.data_ptr(), up.scale.data_ptr(), down.data.data_ptr(),
         down.scale.data_ptr(), L.dt(gate.scale), gate.group_size, y.data_ptr(), L.ptr(ws),
         0 if ws is None else ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),

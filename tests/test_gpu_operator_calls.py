@@ -12,10 +12,11 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover - collected on CPU hosts too
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
+from gpu_helpers import LayerWeights  # noqa: E402
 
 from dispatch_b200 import _lib as L  # noqa: E402
 from dispatch_b200.kernels.block import norm_gate_residual, norm_gate_residual_backward  # noqa: E402
-from dispatch_b200.kernels.grouped_gemm_int4 import grouped_matmul_int4  # noqa: E402
+from dispatch_b200.kernels.grouped_gemm_int4 import expert_ffn_int4, grouped_matmul_int4  # noqa: E402
 from dispatch_b200.kernels.grouping import (  # noqa: E402
     combine_tokens,
     combine_tokens_backward,
@@ -86,6 +87,27 @@ def test_a_dropped_groupings_sizes_read_on_another_stream() -> None:
             torch.full((64,), -1, device=DEV, dtype=torch.int32)
         side.synchronize()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ layers
+
+
+def test_ffn_with_strided_offsets(monkeypatch) -> None:
+    """Their copy lives until the launch, whatever is allocated on the way to it."""
+    w = LayerWeights(256, 192, 4)
+    q = quantize_stacked_weights_int4(StackedExpertWeights(w.gate, w.up, w.down))
+    x = torch.randn(21, 256, device=DEV).to(BF16)
+    off = torch.tensor([0, 3, 3, 10, 21], dtype=torch.int32, device=DEV)
+    want = expert_ffn_int4(x, off, q)
+    word = L.status_word(DEV)
+    made = []
+
+    def allocate(device):
+        made.extend(torch.full((5,), -1, dtype=torch.int32, device=DEV) for _ in range(500))
+        return word
+
+    monkeypatch.setattr(L, "status_word", allocate)
+    assert torch.equal(expert_ffn_int4(x, off.repeat_interleave(2)[::2], q), want) and made
 
 
 # ------------------------------------------------------------------ devices
