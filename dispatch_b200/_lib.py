@@ -66,6 +66,7 @@ class MoeNormDesc(ctypes.Structure):
 
 _SIGNATURES = {
     "moe_abi_version": ([], _i32),
+    "moe_exchange_capture_mode": ([ctypes.POINTER(_i32)], _i32),
     "moe_set_ffn_kernel": ([_i32], _i32),
     "moe_ffn_kernel_auto": ([_i64, _i64, _i64, _i64, _i64, _i32], _i32),
     "moe_status_string": ([_i32], ctypes.c_char_p),
@@ -249,9 +250,32 @@ def check(rc: int, what: str) -> None:
 
 # ---------------------------------------------------------------- device state
 _status: dict[int, torch.Tensor] = {}
-# words that belong to a graph: made where the first call on a device is captured, zeroed by its replays
+# the words of calls captured before any eager one on their device: plain memory made outside the graphs
 _captured_status: dict[int, torch.Tensor] = {}
 _workspaces: dict[tuple[int, int, str], torch.Tensor] = {}
+
+
+def _word(idx: int) -> torch.Tensor:
+    return torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+
+
+def _word_outside_the_capture(idx: int) -> torch.Tensor:
+    """A zero word made while the current stream is being captured, on a stream
+    that is not: zeroed once, now, and not again by each replay, which would
+    clear what another graph has reported."""
+    mode = ctypes.c_int(2)  # relaxed: this thread may allocate and synchronise meanwhile
+    check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "status_word")
+    try:
+        for _ in range(64):  # the pool's streams come round, the captured one among them
+            side = torch.cuda.Stream(idx)
+            with torch.cuda.stream(side):
+                if not torch.cuda.is_current_stream_capturing():
+                    word = _word(idx)
+                    side.synchronize()
+                    return word
+    finally:
+        check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "status_word")
+    raise RuntimeError("status_word: no stream outside the capture")
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -259,11 +283,11 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     s = _status.get(idx)
     if s is None:
-        words = _captured_status if torch.cuda.is_current_stream_capturing() else _status
+        capturing = torch.cuda.is_current_stream_capturing()
+        words = _captured_status if capturing else _status
         s = words.get(idx)
         if s is None:
-            s = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-            words[idx] = s
+            s = words[idx] = _word_outside_the_capture(idx) if capturing else _word(idx)
     return s
 
 

@@ -608,6 +608,14 @@ extern "C" {
 
 int moe_abi_version(void) { return MOE_B200_ABI_VERSION; }
 
+int moe_exchange_capture_mode(int* mode) {
+  CHECK_ARG(mode && *mode >= 0 && *mode <= 2, "capture mode must be 0, 1 or 2");
+  auto m = static_cast<cudaStreamCaptureMode>(*mode);
+  CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&m), "cudaThreadExchangeStreamCaptureMode");
+  *mode = static_cast<int>(m);
+  return MOE_OK;
+}
+
 int moe_set_ffn_kernel(int choice) {
   if (choice != MOE_FFN_KERNEL_AUTO && choice != MOE_FFN_KERNEL_TILED && choice != MOE_FFN_KERNEL_STREAM &&
       choice != MOE_FFN_KERNEL_PAIR && choice != MOE_FFN_KERNEL_WARP)

@@ -111,6 +111,12 @@ int moe_ffn_kernel_auto(int64_t R, int64_t G, int64_t T_shared, int64_t H, int64
 #define MOE_ROUTER_SIGMOID_GROUP 1  /* DeepSeek-V3 group-limited sigmoid top-k */
 
 int moe_abi_version(void);
+/*
+ * Exchanges the calling thread's stream capture mode (cudaStreamCaptureMode:
+ * 0 global, 1 thread local, 2 relaxed) with *mode: for host code that has to
+ * allocate device memory outside a capture which the same thread has begun.
+ */
+int moe_exchange_capture_mode(int* mode);
 const char* moe_status_string(int code);
 /* Message of the last failing call on this host thread ("" if none). */
 const char* moe_last_error(void);

@@ -3,6 +3,7 @@ are replayed in any order, other streams and devices, empty batches."""
 
 from __future__ import annotations
 
+import dataclasses
 
 import pytest
 import torch
@@ -46,6 +47,36 @@ def grouped(t=33, k=6, e=64, h=512, dev=DEV, wdtype=F32):
     x = torch.randn(t, h, generator=g).to(dev, BF16)
     y = torch.randn(t * k, h, generator=g).to(dev, BF16)
     return x, y, w, idx, group_tokens_by_expert(idx, w, e)
+
+
+# ------------------------------------------------------------------ graphs
+def test_errors_of_graphs_captured_before_any_eager_call(monkeypatch) -> None:
+    """Their status word is zero before any replay, keeps what one graph
+    reports when another is replayed, and is cleared by the check alone."""
+    x, _, _, _, good = grouped()
+    pos = good.pos.clone()
+    pos[3] = x.shape[0] * 6  # one past the last row
+    bad = dataclasses.replace(good, pos=pos)
+    permute_tokens(x, good)
+    monkeypatch.setattr(L, "_status", {})
+    monkeypatch.setattr(L, "_captured_status", {})
+    graphs = []
+    for grouping in (good, bad):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = permute_tokens(x, grouping)
+        graphs.append((g, out))
+    L.check_device_status(DEV)  # neither has run
+    (ok, xs), (wrong, _) = graphs
+    for order in ((wrong,), (wrong, ok), (ok, wrong)):
+        for g in order:
+            g.replay()
+        with pytest.raises(L.MoeDeviceError, match="positions out of range"):
+            L.check_device_status(DEV)
+        L.check_device_status(DEV)
+    ok.replay()
+    L.check_device_status(DEV)
+    assert torch.equal(xs, permute_tokens(x, good))
 
 
 # ------------------------------------------------------------------ streams
