@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().with_name("libmoe_b200.so")
 
@@ -221,11 +222,23 @@ def call(what: str, device: torch.device, fn, *args) -> None:
         check(rc, what)
 
 
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises for a tensor that carries a forward-mode derivative: it does not
+    require grad, its values are readable, and its tangent would be lost."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside any dual_level, where none is valid
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: forward-mode derivatives are not implemented")
+
+
 def grad_wanted(what: str, *tensors: torch.Tensor | None) -> bool:
     """Whether autograd has to record this call. Refused while a CUDA graph is
     being captured: autograd's own stream bookkeeping for the leaves is not
     part of the capture, and a captured backward of leaves that an eager graph
-    also holds ends the process. The explicit ``*_backward`` calls capture."""
+    also holds ends the process. The explicit ``*_backward`` calls capture.
+    Forward-mode derivatives are refused."""
+    refuse_tangents(what, *tensors)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return False
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():

@@ -26,6 +26,7 @@ def _check_activations(x: torch.Tensor, q: Int4Tensor) -> None:
         raise ValueError(f"K mismatch: x has {tuple(x.shape)}, qweight has K={q.k}")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"dtype mismatch: activations must be bf16/f16, got {x.dtype}")
+    L.refuse_tangents("the int4 products", x)
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("int4 weights are for inference: call under torch.no_grad() or detach x")
 

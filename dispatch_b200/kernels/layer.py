@@ -117,6 +117,7 @@ def moe_layer_forward(
 def _layer_int4(x, router_weight, weights, router, shared, e_score_bias, topk, out_dtype) -> LayerOutput:
     """The layer with 4-bit experts: the same route, grouping and combine
     kernels around the int4 products, call by call."""
+    L.refuse_tangents("moe_layer_forward", x, *(topk or ()))
     act = act_dtype_for(x, weights)
     if shared is not None and x.dtype != act:
         raise ValueError("the shared expert needs x in the activation dtype")
@@ -170,6 +171,7 @@ def moe_block_forward(  # noqa: PLR0913
     ``norm_gate_residual``."""
     if (normed is None) == (pre_weight is None):
         raise ValueError("give pre_weight or normed, not both")
+    L.refuse_tangents("moe_block_forward", x, pre_weight, normed, post_weight, next_weight, gate)
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, pre_weight, normed, post_weight, next_weight, gate)):
         raise ValueError("moe_block_forward is for inference: call it under torch.no_grad()")

@@ -7,6 +7,7 @@ import dataclasses
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -16,7 +17,7 @@ if not torch.cuda.is_available():  # pragma: no cover - collected on CPU hosts t
 from gpu_helpers import LayerWeights  # noqa: E402
 
 from dispatch_b200 import _lib as L  # noqa: E402
-from dispatch_b200.kernels.block import norm_gate_residual, norm_gate_residual_backward  # noqa: E402
+from dispatch_b200.kernels.block import norm_gate_residual, norm_gate_residual_backward, rms_norm  # noqa: E402
 from dispatch_b200.kernels.grouped_gemm_int4 import expert_ffn_int4, grouped_matmul_int4  # noqa: E402
 from dispatch_b200.kernels.grouping import (  # noqa: E402
     combine_tokens,
@@ -118,6 +119,22 @@ def test_a_dropped_groupings_sizes_read_on_another_stream() -> None:
             torch.full((64,), -1, device=DEV, dtype=torch.int32)
         side.synchronize()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ derivatives
+def test_forward_mode_derivatives_are_refused() -> None:
+    x, y, w, _, grouping = grouped()
+    weight = torch.ones(512, device=DEV)
+    q = pack_int4(torch.zeros(1, 16, 512, dtype=torch.int8, device=DEV), torch.ones(1, 16, 4, device=DEV), 128)
+    calls = [(lambda d: rms_norm(d, weight), x), (lambda d: rms_norm(x, d), weight),
+             (lambda d: norm_gate_residual(x, d, weight), x), (lambda d: permute_tokens(d, grouping), x),
+             (lambda d: combine_tokens(d, grouping, w), y), (lambda d: combine_tokens(y, grouping, d), w),
+             (lambda d: grouped_matmul_int4(d, q, build_tile_schedule(torch.tensor([33]), 16)), x)]
+    with forward_ad.dual_level():
+        for call, t in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            call(t)  # an ordinary tensor inside the level
 
 
 # ------------------------------------------------------------------ layers

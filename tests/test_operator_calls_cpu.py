@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from dispatch_b200 import _lib as L
 from dispatch_b200.kernels.layer import RouterConfig, moe_block_forward, moe_layer_forward
@@ -66,6 +67,26 @@ def test_ffn_without_a_scale_is_refused(missing) -> None:
                                  scale["down_scale"], L.DT_F32, 32, at, at,
                                  lib.moe_ffn_int4_workspace_bytes(8, E, H, I, 32), None, None)
     assert rc == L.MOE_ERR_INVALID_ARG and b"null" in lib.moe_last_error()
+
+
+# ------------------------------------------------------------------ derivatives
+def test_forward_mode_derivatives_are_refused() -> None:
+    """A dual tensor does not require grad, and its tangent would be lost."""
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        assert not dual.requires_grad
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode"):
+                L.grad_wanted("op", None, dual)
+        assert not L.grad_wanted("op", x)
+        q = Int4StackedExpertWeights(int4(), int4(), int4(n=H, k=I))
+        dual = forward_ad.make_dual(torch.zeros(T, H, dtype=BF16), torch.zeros(T, H, dtype=BF16))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            moe_layer_forward(dual, None, q, RouterConfig(top_k=K), topk=topk())
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            moe_block_forward(dual, None, None, q, RouterConfig(top_k=K), normed=dual, topk=topk())
+    assert not L.grad_wanted("op", x) and L.grad_wanted("op", x.clone().requires_grad_())
 
 
 # ------------------------------------------------------------------ weights
