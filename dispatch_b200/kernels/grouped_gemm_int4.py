@@ -18,6 +18,14 @@ from dispatch_b200.kernels.quantization import Int4StackedExpertWeights, Int4Ten
 from dispatch_b200.kernels.tile_schedule import TileSchedule, device_offsets
 
 
+def refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
+    """4-bit weights are frozen and no product has a backward: raises for an
+    input whose derivative would be lost."""
+    L.refuse_tangents(what, *tensors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what}: int4 weights are for inference: call under torch.no_grad() or detach the inputs")
+
+
 def _check_activations(x: torch.Tensor, q: Int4Tensor) -> None:
     if not (x.is_cuda and q.data.is_cuda and q.scale.is_cuda):
         raise ValueError("the B200 int4 grouped-GEMM kernels need CUDA tensors")
@@ -26,9 +34,7 @@ def _check_activations(x: torch.Tensor, q: Int4Tensor) -> None:
         raise ValueError(f"K mismatch: x has {tuple(x.shape)}, qweight has K={q.k}")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"dtype mismatch: activations must be bf16/f16, got {x.dtype}")
-    L.refuse_tangents("the int4 products", x)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("int4 weights are for inference: call under torch.no_grad() or detach x")
+    refuse_gradients("the int4 products", x)
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:

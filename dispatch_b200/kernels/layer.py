@@ -15,6 +15,7 @@ import torch
 
 from dispatch_b200 import _lib as L
 from dispatch_b200.kernels.block import norm_gate_residual, rms_norm
+from dispatch_b200.kernels.grouped_gemm_int4 import refuse_gradients
 from dispatch_b200.kernels.grouping import _group, combine
 from dispatch_b200.kernels.moe_forward import SharedExpertWeights, StackedExpertWeights, act_dtype_for, expert_ffn
 from dispatch_b200.kernels.quantization import Int4StackedExpertWeights, QuantizedStackedExpertWeights
@@ -117,7 +118,7 @@ def moe_layer_forward(
 def _layer_int4(x, router_weight, weights, router, shared, e_score_bias, topk, out_dtype) -> LayerOutput:
     """The layer with 4-bit experts: the same route, grouping and combine
     kernels around the int4 products, call by call."""
-    L.refuse_tangents("moe_layer_forward", x, *(topk or ()))
+    refuse_gradients("moe_layer_forward", x, None if topk is None else topk[1])
     act = act_dtype_for(x, weights)
     if shared is not None and x.dtype != act:
         raise ValueError("the shared expert needs x in the activation dtype")

@@ -205,6 +205,11 @@ def act_dtype_for(x: torch.Tensor, weights) -> torch.dtype:
 
 
 def _routed_forward(x, topk_idx, topk_weight, weights, shared: SharedExpertWeights | None) -> torch.Tensor:
+    from dispatch_b200.kernels.grouped_gemm_int4 import refuse_gradients  # noqa: PLC0415
+    from dispatch_b200.kernels.quantization import Int4StackedExpertWeights  # noqa: PLC0415
+
+    if isinstance(weights, Int4StackedExpertWeights):
+        refuse_gradients("the routed experts", x, topk_weight)
     if topk_idx.shape != topk_weight.shape:
         raise ValueError(
             f"topk_idx.shape {tuple(topk_idx.shape)} != topk_weight.shape {tuple(topk_weight.shape)}"

@@ -85,8 +85,24 @@ def test_forward_mode_derivatives_are_refused() -> None:
         with pytest.raises(RuntimeError, match="forward-mode"):
             moe_layer_forward(dual, None, q, RouterConfig(top_k=K), topk=topk())
         with pytest.raises(RuntimeError, match="forward-mode"):
+            grouped_moe_routed_quantized(dual, *topk(), q)
+        with pytest.raises(RuntimeError, match="forward-mode"):
             moe_block_forward(dual, None, None, q, RouterConfig(top_k=K), normed=dual, topk=topk())
     assert not L.grad_wanted("op", x) and L.grad_wanted("op", x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_gradients_of_4_bit_layers_are_refused(which) -> None:
+    x, (idx, w), q = torch.zeros(T, H, dtype=BF16), topk(), weights("int4")
+    (x if which == "x" else w).requires_grad_()
+    with pytest.raises(ValueError, match="inference"):
+        moe_layer_forward(x, None, q, RouterConfig(top_k=K), topk=(idx, w))
+    with pytest.raises(ValueError, match="inference"):
+        grouped_moe_routed_quantized(x, idx, w, q)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        moe_layer_forward(x, None, q, RouterConfig(top_k=K), topk=(idx, w))
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        grouped_moe_routed_quantized(x, idx, w, q)
 
 
 # ------------------------------------------------------------------ weights
