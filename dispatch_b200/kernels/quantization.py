@@ -87,15 +87,14 @@ def grouped_moe_routed_quantized(
     shared=None,
 ) -> torch.Tensor:
     """Reference: quantization.py:92-107. Runs the fused int8 path (two tcgen05
-    launches with in-smem dequantisation), or with 4-bit weights the int4 path
-    (grouped_gemm_int4.py), whatever ``matmul`` is given."""
+    launches with in-smem dequantisation), with 4-bit weights the int4 path
+    (grouped_gemm_int4.py), with ``StackedExpertWeights`` the 16-bit one,
+    whatever ``matmul`` is given."""
     from dispatch_b200.kernels.moe_forward import _routed_forward  # noqa: PLC0415
 
     _check_matmul(matmul)
     if block_m <= 0:
         raise ValueError(f"block_m must be positive, got {block_m}")
-    if not isinstance(weights, (QuantizedStackedExpertWeights, Int4StackedExpertWeights)):
-        raise TypeError(f"expected quantised expert weights, got {type(weights).__name__}")
     return _routed_forward(x, topk_idx, topk_weight, weights, shared)
 
 

@@ -27,8 +27,12 @@ from dispatch_b200.kernels.grouping import (  # noqa: E402
     permute_tokens_backward,
 )
 from dispatch_b200.kernels.layer import RouterConfig, moe_layer_forward  # noqa: E402
-from dispatch_b200.kernels.moe_forward import StackedExpertWeights  # noqa: E402
-from dispatch_b200.kernels.quantization import pack_int4, quantize_stacked_weights_int4  # noqa: E402
+from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed  # noqa: E402
+from dispatch_b200.kernels.quantization import (  # noqa: E402
+    grouped_moe_routed_quantized,
+    pack_int4,
+    quantize_stacked_weights_int4,
+)
 from dispatch_b200.kernels.tile_schedule import build_tile_schedule  # noqa: E402
 
 DEV = torch.device("cuda", 0)
@@ -138,6 +142,11 @@ def test_forward_mode_derivatives_are_refused() -> None:
 
 
 # ------------------------------------------------------------------ layers
+def test_16_bit_weights_in_the_quantised_call() -> None:
+    w = LayerWeights(256, 192, 16)
+    weights = StackedExpertWeights(w.gate, w.up, w.down)
+    x, _, wt, idx, _ = grouped(t=19, k=4, e=16, h=256)
+    assert torch.equal(grouped_moe_routed_quantized(x, idx, wt, weights), grouped_moe_routed(x, idx, wt, weights))
 
 
 def test_ffn_with_strided_offsets(monkeypatch) -> None:

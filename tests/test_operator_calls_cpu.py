@@ -106,6 +106,9 @@ def test_gradients_of_4_bit_layers_are_refused(which) -> None:
 
 
 # ------------------------------------------------------------------ weights
+def test_16_bit_weights_reach_the_quantised_call() -> None:
+    with pytest.raises(ValueError, match="CUDA"):
+        grouped_moe_routed_quantized(torch.zeros(T, H, dtype=BF16), *topk(), weights("bf16"))
 
 
 def test_the_exact_flag_travels_with_the_weights() -> None:
