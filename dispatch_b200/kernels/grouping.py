@@ -147,11 +147,12 @@ def _row_view(t: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 
 def _weights(what: str, topk_weight: torch.Tensor | None, grouping: TokenGrouping) -> torch.Tensor:
-    """(T*k) weights in their own type."""
+    """The weights, (T, k) or flat, in their own type."""
     if topk_weight is None:
         return grouping.flat_weight
-    if topk_weight.numel() != grouping.pos.numel():
-        raise ValueError(f"{what}: topk_weight has {topk_weight.numel()} values, grouping describes {grouping.pos.numel()}")
+    n, k = grouping.pos.numel(), grouping.top_k
+    if topk_weight.shape not in ((n // k, k), (n,)):
+        raise ValueError(f"{what}: topk_weight.shape {tuple(topk_weight.shape)}, grouping describes ({n // k}, {k})")
     return topk_weight if topk_weight.is_contiguous() else topk_weight.detach().contiguous()
 
 

@@ -8,6 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from dispatch_b200 import _lib as L
+from dispatch_b200.kernels.grouping import TokenGrouping, combine_tokens, combine_tokens_backward
 from dispatch_b200.kernels.layer import RouterConfig, moe_block_forward, moe_layer_forward
 from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed
 from dispatch_b200.kernels.quantization import (
@@ -109,6 +110,22 @@ def test_gradients_of_4_bit_layers_are_refused(which) -> None:
 def test_16_bit_weights_reach_the_quantised_call() -> None:
     with pytest.raises(ValueError, match="CUDA"):
         grouped_moe_routed_quantized(torch.zeros(T, H, dtype=BF16), *topk(), weights("bf16"))
+
+
+def test_weights_of_another_order_are_refused() -> None:
+    """(T, k) or flat: a transposed matrix has as many values."""
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    grouping = TokenGrouping(torch.zeros(T * K, dtype=torch.int64), torch.ones(T * K), torch.zeros(E, dtype=torch.int64),
+                             i32(E + 1), i32(T * K), torch.ones(T * K), K)
+    y, dout = torch.zeros(T * K, H), torch.zeros(T, H)
+    for w in (torch.ones(K, T), torch.ones(T, K, 1), torch.ones(1, T * K)):
+        with pytest.raises(ValueError, match="topk_weight"):
+            combine_tokens(y, grouping, w)
+    for w in (torch.ones(T, K), torch.ones(T * K)):
+        with pytest.raises(ValueError, match="CUDA"):
+            combine_tokens(y, grouping, w)
+        with pytest.raises(ValueError, match="CUDA"):
+            combine_tokens_backward(dout, y, grouping, w)
 
 
 def test_the_exact_flag_travels_with_the_weights() -> None:
