@@ -171,16 +171,21 @@ def _expert_ffn_int4(xs, offsets, weights, shared: SharedExpertWeights | None, x
 
     if gather_rows is not None:
         raise ValueError("int4 experts take no gathered rows")
+    if shared is not None:
+        if x_shared is None:
+            raise ValueError("shared expert needs x_shared")
+        act, h, i_sh = xs.dtype, xs.shape[1], shared.gate.shape[0]
+        if not (shared.gate.dtype == shared.up.dtype == shared.down.dtype == x_shared.dtype == act):
+            raise ValueError(f"dtype mismatch: shared expert must be {act}")
+        if (x_shared.dim() != 2 or x_shared.shape[1] != h or shared.down.shape != (h, i_sh)
+                or not (shared.gate.shape == shared.up.shape == (i_sh, h))):
+            raise ValueError(f"shared expert: x has {tuple(x_shared.shape)}, weights are gate {tuple(shared.gate.shape)} "
+                             f"up {tuple(shared.up.shape)} down {tuple(shared.down.shape)}")
     y = expert_ffn_int4(xs, offsets, weights)
     if shared is None:
         return y, None
-    if x_shared is None:
-        raise ValueError("shared expert needs x_shared")
-    act, h = xs.dtype, xs.shape[1]
-    if shared.gate.dtype != act or x_shared.dtype != act:
-        raise ValueError(f"dtype mismatch: shared expert must be {act}")
     dev = L.require_cuda(xs, x_shared, shared.gate, shared.up, shared.down, what="the B200 expert FFN")
-    t, i_sh = x_shared.shape[0], shared.gate.shape[0]
+    t = x_shared.shape[0]
     ys = torch.empty(t, h, dtype=act, device=dev)
     lib = L.lib()
     ws = torch.empty(max(lib.moe_ffn_workspace_bytes(0, 0, t, i_sh), 256), dtype=torch.uint8, device=dev)

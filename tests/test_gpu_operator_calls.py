@@ -27,7 +27,7 @@ from dispatch_b200.kernels.grouping import (  # noqa: E402
     permute_tokens_backward,
 )
 from dispatch_b200.kernels.layer import RouterConfig, moe_layer_forward  # noqa: E402
-from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed  # noqa: E402
+from dispatch_b200.kernels.moe_forward import SharedExpertWeights, StackedExpertWeights, grouped_moe_routed  # noqa: E402
 from dispatch_b200.kernels.quantization import (  # noqa: E402
     grouped_moe_routed_quantized,
     pack_int4,
@@ -147,6 +147,15 @@ def test_16_bit_weights_in_the_quantised_call() -> None:
     weights = StackedExpertWeights(w.gate, w.up, w.down)
     x, _, wt, idx, _ = grouped(t=19, k=4, e=16, h=256)
     assert torch.equal(grouped_moe_routed_quantized(x, idx, wt, weights), grouped_moe_routed(x, idx, wt, weights))
+
+
+def test_a_4_bit_layer_without_tokens() -> None:
+    w = LayerWeights(256, 192, 16, 320)
+    q = quantize_stacked_weights_int4(StackedExpertWeights(w.gate, w.up, w.down), group_size=64)
+    x = torch.empty(0, 256, device=DEV, dtype=BF16)
+    for shared in (None, SharedExpertWeights(*w.shared)):
+        out = moe_layer_forward(x, w.router, q, RouterConfig(top_k=4), shared=shared)
+        assert out.out.shape == (0, 256) and out.topk_idx.shape == (0, 4) and not out.group_offsets.any()
 
 
 def test_ffn_with_strided_offsets(monkeypatch) -> None:

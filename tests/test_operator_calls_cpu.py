@@ -10,7 +10,7 @@ from torch.autograd import forward_ad
 from dispatch_b200 import _lib as L
 from dispatch_b200.kernels.grouping import TokenGrouping, combine_tokens, combine_tokens_backward
 from dispatch_b200.kernels.layer import RouterConfig, moe_block_forward, moe_layer_forward
-from dispatch_b200.kernels.moe_forward import StackedExpertWeights, grouped_moe_routed
+from dispatch_b200.kernels.moe_forward import SharedExpertWeights, StackedExpertWeights, expert_ffn, grouped_moe_routed
 from dispatch_b200.kernels.quantization import (
     Int4StackedExpertWeights,
     Int4Tensor,
@@ -110,6 +110,19 @@ def test_gradients_of_4_bit_layers_are_refused(which) -> None:
 def test_16_bit_weights_reach_the_quantised_call() -> None:
     with pytest.raises(ValueError, match="CUDA"):
         grouped_moe_routed_quantized(torch.zeros(T, H, dtype=BF16), *topk(), weights("bf16"))
+
+
+@pytest.mark.parametrize("shared", [
+    SharedExpertWeights(torch.zeros(8, H, dtype=BF16), torch.zeros(16, H, dtype=BF16), torch.zeros(H, 8, dtype=BF16)),
+    SharedExpertWeights(torch.zeros(8, 32, dtype=BF16), torch.zeros(8, 32, dtype=BF16), torch.zeros(32, 8, dtype=BF16)),
+    SharedExpertWeights(torch.zeros(8, H, dtype=BF16), torch.zeros(8, H, dtype=BF16), torch.zeros(8, H, dtype=BF16)),
+    SharedExpertWeights(torch.zeros(8, H, dtype=BF16), torch.zeros(8, H), torch.zeros(H, 8, dtype=BF16)),
+])
+def test_a_shared_expert_that_does_not_fit_the_4_bit_ones_is_refused(shared) -> None:
+    x = torch.zeros(T, H, dtype=BF16)
+    off = torch.tensor([0, T, T, T, T], dtype=torch.int32)
+    with pytest.raises(ValueError, match="shared expert"):
+        expert_ffn(x, off, weights("int4"), shared, x)
 
 
 def test_weights_of_another_order_are_refused() -> None:
