@@ -62,8 +62,11 @@ __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t b
 }
 
 // The A operand of one MMA step from its word of eight codes u = code + 8,
-// exactly: a nibble under an exponent's mantissa is a float 2^m + u, from which
-// 2^m + 8 is subtracted.
+// exactly: a nibble put into the mantissa of 2^m is the float 2^m + u, from which
+// 2^m + 8 is subtracted (published for integer weights by Kim, Henry, Fahim and
+// Awadalla, "Who Says Elephants Can't Run: Bringing Large Scale MoE Models into
+// Cloud Scale Production", 2022). m = 10 and 7 are the mantissas' lengths, so the
+// mantissa's last bit counts 1; f16's longer one also takes the nibble 4 bits higher.
 template <bool kF16>
 __device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4]) {
   if (kF16) {
@@ -79,7 +82,7 @@ __device__ __forceinline__ void codes_to_a(uint32_t w, uint32_t (&a)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = and_or(i ? w >> (4 * i) : w, 0x000F000Fu, 0x43004300u);  // 128 + u
-      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(a[i]) : "r"(v), "r"(0x3F803F80u), "r"(0xC308C308u));  // * 1 - 136
+      asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(a[i]) : "r"(v), "r"(0x43084308u));  // - 136
     }
   }
 }
