@@ -98,9 +98,10 @@ def combine(y: torch.Tensor, pos: torch.Tensor, flat_weight: torch.Tensor, num_t
     ys = None if y_shared is None else y_shared.contiguous()
     if ys is not None and ys.dtype != y.dtype:
         ys = ys.to(y.dtype)
+    y, flat_weight = y.contiguous(), flat_weight.contiguous()
     L.call(
         "ungroup_and_combine", dev, L.lib().moe_combine,
-        y.contiguous().data_ptr(), L.dt(y), pos.data_ptr(), flat_weight.contiguous().data_ptr(), num_tokens,
+        y.data_ptr(), L.dt(y), pos.data_ptr(), flat_weight.data_ptr(), num_tokens,
         top_k, h, L.ptr(ys), out.data_ptr(), L.dt(out), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
     return out

@@ -100,14 +100,17 @@ def moe_layer_forward(
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
     rw = None if router_weight is None else router_weight.contiguous()
     sc = (weights.gate.scale, weights.up.scale, weights.down.scale) if quant else (None, None, None)
+    # copies, where these are strided, that live until the launch
+    g, u, dn = g.contiguous(), u.contiguous(), dn.contiguous()
+    sh = (None,) * 3 if shared is None else tuple(w.contiguous() for w in (shared.gate, shared.up, shared.down))
+    bias = None if e_score_bias is None else e_score_bias.contiguous()
     L.call(
         "moe_layer_forward", dev, lib.moe_layer_forward,
-        ctypes.byref(desc), x.data_ptr(), L.ptr(rw), L.ptr(e_score_bias),
+        ctypes.byref(desc), x.data_ptr(), L.ptr(rw), L.ptr(bias),
         L.ptr(idx_in), L.ptr(w_in),
-        g.contiguous().data_ptr(), u.contiguous().data_ptr(), dn.contiguous().data_ptr(),
+        g.data_ptr(), u.data_ptr(), dn.data_ptr(),
         L.ptr(sc[0]), L.ptr(sc[1]), L.ptr(sc[2]),
-        L.ptr(None if shared is None else shared.gate), L.ptr(None if shared is None else shared.up),
-        L.ptr(None if shared is None else shared.down),
+        *map(L.ptr, sh),
         out.data_ptr(), None if topk is not None else idx.data_ptr(), None if topk is not None else wts.data_ptr(),
         counts.data_ptr(), offsets.data_ptr(), ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(),
         L.stream_ptr(dev),

@@ -148,17 +148,18 @@ def expert_ffn(xs: torch.Tensor, offsets: torch.Tensor, weights, shared: SharedE
     nbytes = lib.moe_ffn_workspace_bytes(r, i, t_sh, i_sh)
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
     sc = (weights.gate.scale, weights.up.scale, weights.down.scale) if quant else (None, None, None)
+    # copies, where these are strided, that live until the launch
+    g, u, d = g.contiguous(), u.contiguous(), d.contiguous()
+    sh = (None,) * 3 if shared is None else tuple(w.contiguous() for w in (shared.gate, shared.up, shared.down))
     L.call(
         "expert_ffn", dev, lib.moe_expert_ffn_grouped,
         3, xs.data_ptr(), L.dt(act), r, h, offsets.data_ptr(), e, e,
         L.ptr(gather_rows), xs.shape[0] if gather_rows is not None else 0, i,
-        g.contiguous().data_ptr(), u.contiguous().data_ptr(), d.contiguous().data_ptr(),
+        g.data_ptr(), u.data_ptr(), d.data_ptr(),
         L.DT_I8 if quant else L.dt(act),
         L.ptr(sc[0]), L.ptr(sc[1]), L.ptr(sc[2]), L.dt(sc[0]) if quant else 0,
         L.ptr(x_shared), t_sh, i_sh,
-        L.ptr(None if shared is None else shared.gate.contiguous()),
-        L.ptr(None if shared is None else shared.up.contiguous()),
-        L.ptr(None if shared is None else shared.down.contiguous()),
+        *map(L.ptr, sh),
         y.data_ptr(), L.ptr(ys), ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
     )
     return y, ys

@@ -149,6 +149,21 @@ def test_16_bit_weights_in_the_quantised_call() -> None:
     assert torch.equal(grouped_moe_routed_quantized(x, idx, wt, weights), grouped_moe_routed(x, idx, wt, weights))
 
 
+def test_strided_weights() -> None:
+    """Their copies live until the launch, each in memory of its own."""
+    w = LayerWeights(256, 192, 16, 320)
+    x, _, wt, idx, _ = grouped(t=19, k=4, e=16, h=256)
+    strided = lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+    plain = StackedExpertWeights(w.gate, w.up, w.down), SharedExpertWeights(*w.shared)
+    other = StackedExpertWeights(*map(strided, (w.gate, w.up, w.down))), SharedExpertWeights(*map(strided, w.shared))
+    cfg = RouterConfig(top_k=4)
+    for shared in (False, True):
+        a, b = (moe_layer_forward(x, w.router, p[0], cfg, shared=p[1] if shared else None).out for p in (plain, other))
+        assert torch.equal(a, b)
+        a, b = (grouped_moe_routed(x, idx, wt, p[0], shared=p[1] if shared else None) for p in (plain, other))
+        assert torch.equal(a, b)
+
+
 def test_a_4_bit_layer_without_tokens() -> None:
     w = LayerWeights(256, 192, 16, 320)
     q = quantize_stacked_weights_int4(StackedExpertWeights(w.gate, w.up, w.down), group_size=64)
