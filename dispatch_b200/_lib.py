@@ -272,23 +272,22 @@ def _word(idx: int) -> torch.Tensor:
     return torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
 
 
-def _word_outside_the_capture(idx: int) -> torch.Tensor:
-    """A zero word made while the current stream is being captured, on a stream
-    that is not: zeroed once, now, and not again by each replay, which would
-    clear what another graph has reported."""
+def outside_the_capture(device: torch.device, make):
+    """``make()`` while the current stream is being captured, but on a stream
+    that is not: done once, now, when this returns, and not by each replay."""
     mode = ctypes.c_int(2)  # relaxed: this thread may allocate and synchronise meanwhile
-    check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "status_word")
+    check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "outside_the_capture")
     try:
         for _ in range(64):  # the pool's streams come round, the captured one among them
-            side = torch.cuda.Stream(idx)
+            side = torch.cuda.Stream(device)
             with torch.cuda.stream(side):
                 if not torch.cuda.is_current_stream_capturing():
-                    word = _word(idx)
+                    made = make()
                     side.synchronize()
-                    return word
+                    return made
     finally:
-        check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "status_word")
-    raise RuntimeError("status_word: no stream outside the capture")
+        check(lib().moe_exchange_capture_mode(ctypes.byref(mode)), "outside_the_capture")
+    raise RuntimeError("no stream outside the capture")
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -300,7 +299,8 @@ def status_word(device: torch.device) -> torch.Tensor:
         words = _captured_status if capturing else _status
         s = words.get(idx)
         if s is None:
-            s = words[idx] = _word_outside_the_capture(idx) if capturing else _word(idx)
+            # zeroed once: a node of the graph would clear what another graph has reported
+            s = words[idx] = outside_the_capture(torch.device("cuda", idx), lambda: _word(idx)) if capturing else _word(idx)
     return s
 
 

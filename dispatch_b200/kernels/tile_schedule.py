@@ -13,6 +13,8 @@ from dataclasses import dataclass
 
 import torch
 
+from dispatch_b200 import _lib as L
+
 
 @dataclass(frozen=True)
 class TileSchedule:
@@ -51,15 +53,49 @@ def build_tile_schedule(group_sizes: torch.Tensor, block_m: int) -> TileSchedule
     return TileSchedule(block_m, tuple(offsets), i32(te), i32(ts), i32(tv))
 
 
+class _Upload:
+    """The offsets of a schedule on a device: what was copied, where, and when."""
+
+    __slots__ = ("values", "tensor", "stream", "done")
+
+    def __init__(self, values: tuple[int, ...], device: torch.device):
+        self.values = values
+        self.tensor = torch.tensor(values, dtype=torch.int32).to(device, non_blocking=True)
+        self.stream, self.done = None, None
+        if device.type == "cuda":
+            self.stream = L.stream_ptr(device)
+            self.done = torch.cuda.Event()
+            self.done.record(torch.cuda.current_stream(device))
+
+    def __reduce__(self):  # a copied or pickled schedule uploads its own
+        return type(None), ()
+
+
+# read by captured graphs at each replay, whatever becomes of the schedule
+_captured_uploads: list[_Upload] = []
+
+
 def device_offsets(schedule, device: torch.device) -> torch.Tensor:
     """``schedule.group_offsets`` as an int32 device tensor (accepts the
-    reference's TileSchedule too: only ``group_offsets`` is read)."""
-    cached = getattr(schedule, "_b200_offsets", None)
-    if cached is not None and cached.device == device:
-        return cached
-    t = torch.tensor(schedule.group_offsets, dtype=torch.int32).to(device, non_blocking=True)
-    try:
-        object.__setattr__(schedule, "_b200_offsets", t)
-    except (AttributeError, TypeError):
-        pass
-    return t
+    reference's TileSchedule too: only ``group_offsets`` is read). Uploaded
+    once per schedule, device and values; other streams wait for the copy, and
+    a captured call's copy is made and finished outside the graph."""
+    offsets = schedule.group_offsets
+    up = getattr(schedule, "_b200_offsets", None)
+    capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    if up is None or up.tensor.device != device or (up.values is not offsets and up.values != tuple(offsets)):
+        values = tuple(offsets)
+        up = L.outside_the_capture(device, lambda: _Upload(values, device)) if capturing else _Upload(values, device)
+        try:
+            object.__setattr__(schedule, "_b200_offsets", up)
+        except (AttributeError, TypeError):
+            pass
+    elif capturing:
+        L.outside_the_capture(device, up.done.synchronize)
+    elif up.done is not None and up.stream != L.stream_ptr(device):
+        here = torch.cuda.current_stream(device)
+        here.wait_event(up.done)
+        up.tensor.record_stream(here)
+    if capturing:
+        _captured_uploads.append(up)
+    return up.tensor

@@ -18,6 +18,7 @@ from gpu_helpers import LayerWeights  # noqa: E402
 
 from dispatch_b200 import _lib as L  # noqa: E402
 from dispatch_b200.kernels.block import norm_gate_residual, norm_gate_residual_backward, rms_norm  # noqa: E402
+from dispatch_b200.kernels.grouped_gemm import grouped_matmul  # noqa: E402
 from dispatch_b200.kernels.grouped_gemm_int4 import expert_ffn_int4, grouped_matmul_int4  # noqa: E402
 from dispatch_b200.kernels.grouping import (  # noqa: E402
     combine_tokens,
@@ -84,7 +85,54 @@ def test_errors_of_graphs_captured_before_any_eager_call(monkeypatch) -> None:
     assert torch.equal(xs, permute_tokens(x, good))
 
 
+@pytest.mark.parametrize("first", ["captured", "eager"])
+def test_products_in_a_graph_that_outlives_its_schedule(first) -> None:
+    """The graph reads offsets that were copied before its replay and that
+    nothing else is given; an eager call before the replay reads them too."""
+    x = torch.randn(21, 64, device=DEV).to(BF16)
+    w = torch.randn(4, 32, 64, device=DEV).to(BF16)
+    codes = torch.randint(-8, 8, (4, 32, 64), device=DEV).to(torch.int8)
+    q = pack_int4(codes, torch.ones(4, 32, 1, device=DEV) / 16, 64)
+    sizes = torch.tensor([3, 0, 7, 11])
+    want = grouped_matmul_int4(x, q, build_tile_schedule(sizes, 16)), grouped_matmul(x, w, build_tile_schedule(sizes, 16))
+    sched = build_tile_schedule(sizes, 16)
+    if first == "eager":
+        assert torch.equal(grouped_matmul_int4(x, q, sched), want[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = grouped_matmul_int4(x, q, sched), grouped_matmul(x, w, sched)
+    assert torch.equal(grouped_matmul_int4(x, q, sched), want[0])
+    del sched
+    for _ in range(200):
+        torch.full((5,), -1, dtype=torch.int32, device=DEV)
+    for _ in range(2):
+        for t in got:
+            t.zero_()
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------ streams
+def test_a_schedule_used_on_another_stream() -> None:
+    """Its offsets are copied behind whatever the first stream is doing, and the second stream waits for the copy."""
+    x = torch.randn(21, 64, device=DEV).to(BF16)
+    q = pack_int4(torch.ones(4, 32, 64, dtype=torch.int8, device=DEV), torch.ones(4, 32, 1, device=DEV) / 16, 64)
+    sizes = torch.tensor([3, 0, 7, 11])
+    want = grouped_matmul_int4(x, q, build_tile_schedule(sizes, 16))
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        sched = build_tile_schedule(sizes, 16)
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(2_000_000)
+            first = grouped_matmul_int4(x, q, sched)
+        with torch.cuda.stream(b):
+            second = grouped_matmul_int4(x, q, sched)
+        del sched
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+
+
 @pytest.mark.parametrize("wdtype", [F32, BF16])
 def test_sizes_belong_to_the_stream_that_made_them(wdtype) -> None:
     """What a grouping holds is made when it is: reading it elsewhere launches

@@ -3,6 +3,9 @@ let through, before anything runs on a GPU."""
 
 from __future__ import annotations
 
+import copy
+from types import SimpleNamespace
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -17,6 +20,7 @@ from dispatch_b200.kernels.quantization import (
     grouped_moe_routed_quantized,
     pack_int4,
 )
+from dispatch_b200.kernels.tile_schedule import build_tile_schedule, device_offsets
 
 BF16 = torch.bfloat16
 T, K, E, H, I = 6, 2, 4, 64, 32
@@ -139,6 +143,23 @@ def test_weights_of_another_order_are_refused() -> None:
             combine_tokens(y, grouping, w)
         with pytest.raises(ValueError, match="CUDA"):
             combine_tokens_backward(dout, y, grouping, w)
+
+
+# ------------------------------------------------------------------ schedules
+def test_offsets_are_those_of_the_schedule_as_it_is() -> None:
+    """What is uploaded is kept by value: a schedule whose offsets change is uploaded again."""
+    cpu = torch.device("cpu")
+    sched = SimpleNamespace(block_m=16, group_offsets=(0, 3, 7))
+    first = device_offsets(sched, cpu)
+    assert first.tolist() == [0, 3, 7] and device_offsets(sched, cpu) is first
+    sched.group_offsets = (0, 5, 7)
+    assert device_offsets(sched, cpu).tolist() == [0, 5, 7]
+    sched.group_offsets = [0, 1, 7]
+    assert device_offsets(sched, cpu).tolist() == [0, 1, 7]
+    sched.group_offsets[1] = 2
+    assert device_offsets(sched, cpu).tolist() == [0, 2, 7]
+    again = copy.deepcopy(build_tile_schedule(torch.tensor([3, 4]), 16))
+    assert device_offsets(again, cpu).tolist() == [0, 3, 7] and device_offsets(copy.deepcopy(again), cpu).tolist() == [0, 3, 7]
 
 
 def test_the_exact_flag_travels_with_the_weights() -> None:
