@@ -84,6 +84,10 @@ _SIGNATURES = {
         [_p, _i32, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p, _i32, _i64, _p, _i32, _p, _sz, _p, _p],
         _i32,
     ),
+    "moe_group_tokens_sizes": (
+        [_p, _i32, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _p, _i32, _p, _sz, _p, _p],
+        _i32,
+    ),
     "moe_group_tokens_noalloc": (
         [_p, _i32, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p, _i32, _i64, _p, _i32, _p, _p],
         _i32,

@@ -33,6 +33,7 @@ struct Params {
   int E;
   int nchunks;
   int32_t* counts;
+  int64_t* sizes = nullptr;  // the counts once more, may be null
   int32_t* offsets;
   int32_t* pos;
   int64_t* sorted_token_idx;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(kThreads) group_scatter_kernel(const Params p)
         base[e] += off;
         if (c == 0 && blockIdx.y == 0) {
           p.counts[e] = cnt;
+          if (p.sizes) p.sizes[e] = cnt;
           p.offsets[e] = off;
         }
       }

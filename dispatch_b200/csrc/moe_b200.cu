@@ -761,10 +761,11 @@ size_t moe_group_workspace_bytes(int64_t T, int k, int64_t E) {
   return static_cast<size_t>((chunks > 0 ? chunks : 1) * E) * sizeof(int32_t);
 }
 
-int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, int64_t T, int k, int64_t E,
-                     int32_t* counts, int32_t* offsets, int32_t* pos, int64_t* sorted_token_idx,
-                     float* sorted_weight, const void* x, int x_dtype, int64_t H, void* xs, int xs_dtype,
-                     void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+int moe_group_tokens_sizes(const void* topk_idx, int idx_dtype, const float* topk_w, int64_t T, int k, int64_t E,
+                           int32_t* counts, int64_t* sizes, int32_t* offsets, int32_t* pos,
+                           int64_t* sorted_token_idx, float* sorted_weight, const void* x, int x_dtype, int64_t H,
+                           void* xs, int xs_dtype, void* workspace, size_t workspace_bytes, int32_t* status,
+                           void* stream) {
   int sms = 0;
   int rc = device_info(&sms);
   if (rc) return rc;
@@ -784,6 +785,7 @@ int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, i
   const int64_t n = T * k;
   if (n == 0) {
     CUDA_TRY(cudaMemsetAsync(counts, 0, E * sizeof(int32_t), s), "memset counts");
+    if (sizes) CUDA_TRY(cudaMemsetAsync(sizes, 0, E * sizeof(int64_t), s), "memset sizes");
     CUDA_TRY(cudaMemsetAsync(offsets, 0, (E + 1) * sizeof(int32_t), s), "memset offsets");
     return MOE_OK;
   }
@@ -796,6 +798,7 @@ int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, i
   p.E = static_cast<int>(E);
   p.nchunks = static_cast<int>((n + moe::group::kChunk - 1) / moe::group::kChunk);
   p.counts = counts;
+  p.sizes = sizes;
   p.offsets = offsets;
   p.pos = pos;
   p.sorted_token_idx = sorted_token_idx;
@@ -808,6 +811,14 @@ int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, i
   p.hist = static_cast<int32_t*>(workspace);
   p.status = status;
   return launch_grouping(p, sms, s);
+}
+
+int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, int64_t T, int k, int64_t E,
+                     int32_t* counts, int32_t* offsets, int32_t* pos, int64_t* sorted_token_idx,
+                     float* sorted_weight, const void* x, int x_dtype, int64_t H, void* xs, int xs_dtype,
+                     void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return moe_group_tokens_sizes(topk_idx, idx_dtype, topk_w, T, k, E, counts, nullptr, offsets, pos, sorted_token_idx,
+                                sorted_weight, x, x_dtype, H, xs, xs_dtype, workspace, workspace_bytes, status, stream);
 }
 
 }  // extern "C"

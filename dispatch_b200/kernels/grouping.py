@@ -36,7 +36,7 @@ class TokenGrouping:
 
 def _group(topk_idx: torch.Tensor, topk_weight: torch.Tensor | None, n_experts: int,
            x: torch.Tensor | None = None, xs_dtype: torch.dtype | None = None,
-           want_sorted: bool = True):
+           want_sorted: bool = True, sizes: torch.Tensor | None = None):
     dev = L.require_cuda(topk_idx, topk_weight, x, what="token grouping")
     t, k = topk_idx.shape
     idx = topk_idx.contiguous()
@@ -58,8 +58,8 @@ def _group(topk_idx: torch.Tensor, topk_weight: torch.Tensor | None, n_experts: 
     nbytes = lib.moe_group_workspace_bytes(t, k, n_experts)
     ws = L.workspace(dev, nbytes, "group")
     L.call(
-        "group_tokens_by_expert", dev, lib.moe_group_tokens,
-        idx.data_ptr(), L.dt(idx), L.ptr(w), t, k, n_experts, counts.data_ptr(), offsets.data_ptr(),
+        "group_tokens_by_expert", dev, lib.moe_group_tokens_sizes,
+        idx.data_ptr(), L.dt(idx), L.ptr(w), t, k, n_experts, counts.data_ptr(), L.ptr(sizes), offsets.data_ptr(),
         pos.data_ptr(), L.ptr(sti), L.ptr(sw),
         L.ptr(x), L.dt(x) if x is not None else 0, h, L.ptr(xs), L.dt(xs_dtype) if xs is not None else 0,
         ws.data_ptr(), ws.numel(), L.status_word(dev).data_ptr(), L.stream_ptr(dev),
@@ -75,13 +75,15 @@ def group_tokens_by_expert(
         raise ValueError(
             f"topk_idx.shape {tuple(topk_idx.shape)} != topk_weight.shape {tuple(topk_weight.shape)}"
         )
-    counts, offsets, pos, sti, sw, w, _ = _group(topk_idx, topk_weight, n_routed_experts)
-    # made here, on the grouping's own stream: a caller who reads them elsewhere
-    # can then protect them with record_stream, or keep them for a captured graph
+    # sizes and weights are made here, on the grouping's own stream: a caller who
+    # reads them elsewhere can then protect them with record_stream, or keep them
+    # for a captured graph
+    sizes = torch.empty(n_routed_experts, dtype=torch.int64, device=topk_idx.device)
+    _, offsets, pos, sti, sw, w, _ = _group(topk_idx, topk_weight, n_routed_experts, sizes=sizes)
     return TokenGrouping(
         sorted_token_idx=sti,
-        sorted_weight=sw.to(topk_weight.dtype),
-        group_sizes=counts.to(torch.int64),
+        sorted_weight=sw if sw.dtype == topk_weight.dtype else sw.to(topk_weight.dtype),
+        group_sizes=sizes,
         offsets=offsets,
         pos=pos,
         flat_weight=w.reshape(-1),

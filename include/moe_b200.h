@@ -163,6 +163,12 @@ int moe_group_tokens(const void* topk_idx, int idx_dtype, const float* topk_w, i
                      int32_t* counts, int32_t* offsets, int32_t* pos, int64_t* sorted_token_idx,
                      float* sorted_weight, const void* x, int x_dtype, int64_t H, void* xs, int xs_dtype,
                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* moe_group_tokens with the counts as int64 as well: sizes (E), may be NULL. */
+int moe_group_tokens_sizes(const void* topk_idx, int idx_dtype, const float* topk_w, int64_t T, int k, int64_t E,
+                           int32_t* counts, int64_t* sizes, int32_t* offsets, int32_t* pos,
+                           int64_t* sorted_token_idx, float* sorted_weight, const void* x, int x_dtype, int64_t H,
+                           void* xs, int xs_dtype, void* workspace, size_t workspace_bytes, int32_t* status,
+                           void* stream);
 
 /*
  * Token grouping without a workspace argument. It has no counterpart in the
