@@ -22,8 +22,9 @@ def refuse_gradients(what: str, *tensors: torch.Tensor | None) -> None:
     """4-bit weights are frozen and no product has a backward: raises for an
     input whose derivative would be lost."""
     L.refuse_tangents(what, *tensors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what}: int4 weights are for inference: call under torch.no_grad() or detach the inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: int4 weights are for inference: call under torch.no_grad() or detach the inputs")
 
 
 def _check_activations(x: torch.Tensor, q: Int4Tensor) -> None:
