@@ -197,11 +197,13 @@ class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, grouping):
         ctx.grouping, ctx.dtype = grouping, x.dtype
+        ctx.save_for_backward(grouping.pos)  # so that a change in place is noticed
         return _permute(x, grouping)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dxs):
+        ctx.saved_tensors  # raises for what was changed in place
         return permute_tokens_backward(dxs, ctx.grouping, out_dtype=ctx.dtype), None
 
 
@@ -255,14 +257,16 @@ def combine_tokens_backward(
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, topk_weight, y_shared, grouping, out_dtype):
-        ctx.save_for_backward(y, topk_weight)
+        # the grouping's own weights may be the caller's tensor: saved so that a change in place is noticed
+        own = grouping.flat_weight if topk_weight is None else None
+        ctx.save_for_backward(y, topk_weight, own, grouping.pos, grouping.offsets)
         ctx.grouping = grouping
         return _combine(y, grouping, topk_weight, y_shared, out_dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, topk_weight = ctx.saved_tensors
+        y, topk_weight, *_ = ctx.saved_tensors
         need_y, need_w, need_shared = ctx.needs_input_grad[:3]
         dy = dw = None
         if need_y or need_w:

@@ -189,6 +189,23 @@ def test_forward_mode_derivatives_are_refused() -> None:
             call(t)  # an ordinary tensor inside the level
 
 
+@pytest.mark.parametrize("what", ["weights", "grouping's weights", "positions", "rows"])
+def test_inputs_changed_before_the_backward_are_noticed(what) -> None:
+    x, y, w, _, grouping = grouped()
+    y = y.requires_grad_()
+    out = combine_tokens(y, grouping, w if what == "weights" else None)
+    with torch.no_grad():
+        {"weights": w, "grouping's weights": w, "positions": grouping.pos, "rows": y}[what].add_(0)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        out.sum().backward()
+    x = x.requires_grad_()
+    xs = permute_tokens(x, grouping)
+    with torch.no_grad():
+        x.add_(1)  # the gather's gradient does not need it
+    xs.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 6))
+
+
 # ------------------------------------------------------------------ layers
 def test_16_bit_weights_in_the_quantised_call() -> None:
     w = LayerWeights(256, 192, 16)
