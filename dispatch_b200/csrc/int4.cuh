@@ -587,8 +587,15 @@ struct QuantParams {
   int N, K, n16, kb, groups, group;
 };
 
+// The larger one, or NaN if either is (fmaxf gives the other).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // One warp per 16-row tile and group of columns: the absolute maximum of each
-// row's group, scale = max / 7 (1 for a group of zeros) rounded to the scales'
+// row's group (NaN or infinite if one of its weights is: so is the scale then), scale = max / 7 (1 for a group of zeros) rounded to the scales'
 // type, code = round_half_even(w / scale) clamped to -8 .. 7, laid out. Groups
 // of 32 write half a block per warp.
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
@@ -610,9 +617,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
     float m = 0.f;
     if (n < p.N)
       for (int col = col0 + q; col < min(col0 + p.group, p.K); col += 4)
-        m = fmaxf(m, fabsf(norm::load_one(p.w, p.w_dt, (e * p.N + n) * p.K + col)));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m = max_nan(m, fabsf(norm::load_one(p.w, p.w_dt, (e * p.N + n) * p.K + col)));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
     float s = m == 0.f ? 1.0f : m / 7.0f;
     if (p.scale_dt == MOE_DT_BF16) s = __bfloat162float(__float2bfloat16_rn(s));
     else if (p.scale_dt == MOE_DT_F16) s = __half2float(__float2half_rn(s));

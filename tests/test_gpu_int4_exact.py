@@ -26,6 +26,7 @@ from dispatch_b200.kernels.quantization import (  # noqa: E402
     pack_int4,
     quantize_groupwise_int4,
     quantize_stacked_weights_int4,
+    unpack_int4,
 )
 from dispatch_b200.kernels.tile_schedule import build_tile_schedule  # noqa: E402
 
@@ -126,3 +127,25 @@ def test_from_c_without_a_workspace() -> None:
     check_exact(out, x, q, [0, rows])
     assert call(ws.data_ptr(), need - 1) == L.MOE_ERR_INVALID_ARG  # room that is too small is a mistake
     assert q.scale.dtype == F32
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_weights_do_not_become_finite(bad, scale_dtype) -> None:
+    """The quantiser's formula: their group's scale is not finite; every other group is as without them."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(2, 20, 200, generator=g, device=DEV)
+    want = quantize_groupwise_int4(w, group_size=32, scale_dtype=scale_dtype)
+    w[1, 17, 70] = bad  # of group 2
+    got = quantize_groupwise_int4(w, group_size=32, scale_dtype=scale_dtype)
+    scale, sane = unpack_int4(got)[1], unpack_int4(want)[1]
+    hit = torch.zeros_like(scale, dtype=torch.bool)
+    hit[1, 17, 2] = True
+    assert not torch.isfinite(scale[hit]).any() and torch.equal(scale[~hit], sane[~hit])
+    columns = hit.repeat_interleave(32, 2)[..., :200]
+    assert torch.equal(unpack_int4(got)[0][~columns], unpack_int4(want)[0][~columns])
+    x = torch.randn(6, 200, generator=g, device=DEV).to(BF16)
+    out = grouped_matmul_int4(x, got, build_tile_schedule(torch.tensor([3, 3]), 16))
+    assert not torch.isfinite(out[3:, 17]).any()
+    out[3:, 17] = 0
+    assert torch.isfinite(out).all()
