@@ -304,7 +304,8 @@ def status_word(device: torch.device) -> torch.Tensor:
         s = words.get(idx)
         if s is None:
             # zeroed once: a node of the graph would clear what another graph has reported
-            s = words[idx] = outside_the_capture(torch.device("cuda", idx), lambda: _word(idx)) if capturing else _word(idx)
+            dev = torch.device("cuda", idx)
+            s = words[idx] = outside_the_capture(dev, lambda: _word(idx)) if capturing else _word(idx)
     return s
 
 

@@ -595,9 +595,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // One warp per 16-row tile and group of columns: the absolute maximum of each
-// row's group (NaN or infinite if one of its weights is: so is the scale then), scale = max / 7 (1 for a group of zeros) rounded to the scales'
-// type, code = round_half_even(w / scale) clamped to -8 .. 7, laid out. Groups
-// of 32 write half a block per warp.
+// row's group (not finite if one of its weights is not: nor is the scale then),
+// scale = max / 7 (1 for a group of zeros) rounded to the scales' type, code =
+// round_half_even(w / scale) clamped to -8 .. 7, laid out. Groups of 32 write
+// half a block per warp. 64 x 1408 x 2048 bf16 in 352 us (floor 72; each weight
+// is read twice, one value per lane): it runs once per weight.
 __global__ void __launch_bounds__(256) quantize_kernel(const QuantParams p) {
   pdl_trigger();
   pdl_wait();  // before the first global memory access

@@ -1988,11 +1988,12 @@ int log2_of(int64_t v) {
 //   16 bits      127/132/133 152/156/159 153/156/160 154/157/161 156/159/162 156/160/163 158/162/164 181/184/186
 // (192 rows, groups of 128: 236 in 64-row tiles, 224 in 128-row tiles, 181 in 16 bits). Each scale group's sums pass
 // through TMEM, so shorter groups cost the tiles more; the 128-row tile pays for groups of 128 on.
-// One limit serves all groups below 128, though with 64 the 64-row tile stays ahead of the 16-bit form up to about
-// 75 rows (64 rows 109 us against 164, 85 rows 184 against 164). Without a workspace, 16-bit form / tiles:
-//   rows         192       384            (groups of 256 / 128 / 64 / 32)
-//   16 bits      187/188/187/190   240/241/241/245
-//   tiles        181/229/285/476   266/338/529/886
+// One limit serves all groups below 128, though with 64 the 64-row tile stays ahead of the 16-bit form up to about 85
+// rows on average. Without a workspace the tiles take every size; with the same rows for each expert (groups of
+// 256 / 128 / 64 / 32):
+//   rows         64                 192                 384
+//   16 bits      -/-/164/166        187/188/187/190     240/241/241/245
+//   tiles        94/109/109/174     181/229/285/476     266/338/529/886
 enum class Int4Form { kWarp, kTile64, kTile128, k16Bit };
 Int4Form int4_form(int64_t M, int64_t E, int group) {
   if (M <= 12 * E) return Int4Form::kWarp;
